@@ -327,7 +327,7 @@ int crhip_free(void *device_pointer)
 		const hipError_t h = hipMemRelease(r.handle);
 		// The address range is NOT given back (hipMemAddressFree): it stays reserved and unmapped for the life of the process, so that a
 		// stale pointer faults for good - and because a range that was freed and handed out again showed kernels and the copy engines
-		// different contents on this runtime (tools/experiments/r06/vmm_probe.py): a diagnostic mode must not add a hazard of its own.
+		// different contents on this runtime (profiles/r06_vmm_probe.log): a diagnostic mode must not add a hazard of its own.
 		return (int)(e != hipSuccess ? e : u != hipSuccess ? u : h);
 	}
 	return (int)hipFree(device_pointer);

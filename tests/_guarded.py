@@ -14,7 +14,6 @@ import os
 import numpy as np
 
 _hip = None
-KEEP_ADDRESSES = os.environ.get("CRA_GUARDED_KEEP", "1") != "0"
 
 
 class _Location(C.Structure):
@@ -124,7 +123,7 @@ class Guarded:
         self.live = True
         if fill is not None:
             # (a host-side pattern copied in, and the device waited for: hipMemset on such a mapping was seen to land LATE - after a
-            # device-to-host copy issued behind it - on this runtime; tools/experiments/r06/vmm_probe.py)
+            # device-to-host copy issued behind it - on this runtime)
             pattern = np.full(self.mapped, fill, dtype=np.uint8)
             _check(h.hipMemcpy(C.c_void_p(self.first), pattern.ctypes.data_as(C.c_void_p), self.mapped, 1), "hipMemcpy(H2D, fill)")
             _check(h.hipDeviceSynchronize(), "hipDeviceSynchronize")
@@ -154,17 +153,15 @@ class Guarded:
         return out
 
     def close(self):
-        """Unmaps and gives the physical pages back; the ADDRESS RANGE stays reserved for the life of the process (KEEP_ADDRESSES).  On this
+        """Unmaps and gives the physical pages back; the ADDRESS RANGE stays reserved for the life of the process.  On this
         runtime a range that was unmapped, freed and handed out again by the next hipMemAddressReserve showed kernels, hipMemset and the
-        copy engines DIFFERENT contents - some of them still translating through the old mapping (tools/experiments/r06/vmm_probe.py,
-        profiles/r06_vmm_probe.log: 16 of 48 buffers bad with reuse, 0 of 48 without).  A test allocator must not add a hazard of its own."""
+        copy engines DIFFERENT contents - some of them still translating through the old mapping
+        (profiles/r06_vmm_probe.log: 16 of 48 buffers bad with reuse, 0 of 48 without).  A test allocator must not add a hazard of its own."""
         if self.live:
             h = hip()
             h.hipDeviceSynchronize()
             h.hipMemUnmap(C.c_void_p(self.first), self.mapped)
             h.hipMemRelease(self.handle)
-            if not KEEP_ADDRESSES:
-                h.hipMemAddressFree(self.base, self.reserved)
             self.live = False
 
     def __enter__(self):

@@ -1,7 +1,7 @@
 #!/bin/bash
 # Round 6 evidence, one box, ONE library build (the PMC summaries are stamped with its source id; bench.py quotes them only for that build):
 # bench lines + rocprofv3 kernel traces for the BASELINE configurations with the mean over the TIMED dispatches taken from the trace
-# (tools/trace_timed_mean.py), PMC passes for them, the long-window shapes' lines, the host paths; then the GPU suite in a loop of fresh processes.
+# (tools/trace_timed_mean.py), PMC passes for them, the long-window shapes' lines, the host paths.
 #   gpurun --timeout 3300 -- 'bash tools/r06_final_profiles.sh'     then     python tools/r06_install_evidence.py
 set -u
 cd /tmp; export TMPDIR=/tmp
@@ -38,4 +38,3 @@ print("$w", l["roofline"]["kernel"], "%.1f us" % (l["ms_per_step"]*1e3), "median
 PY
 done | tee $O/lines.log
 rm -f $O/*.err
-bash tools/experiments/r06/loop_suite.sh d ${LOOP_RUNS:-12}
