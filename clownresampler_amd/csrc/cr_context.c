@@ -377,6 +377,8 @@ static unsigned long long g_launch_count[CR_KERNEL_IDS];
 #define CR_SEG_MAX_WASTE 0.06
 /* consecutive tiles an XCD takes per round (crhip_seg_launch.xcd_run; cr_kseg.hpp): neighbouring tiles read neighbouring bytes of the same input lines */
 #define CR_SEG_XCD_RUN 16
+/* the largest copy between the device and pageable host memory (copy_pageable_h2d) */
+#define CR_PAGEABLE_PIECE ((size_t)1 << 20)
 /* a launch of a periodic ratio that starts mid-period is split (a few frames on the ordinary kernel, the rest on k_int) from this
    many output frames on: below, the second launch costs more than k_int saves */
 #define CR_INT_SPLIT_MIN_FRAMES 8192u
@@ -403,6 +405,7 @@ static struct
 	int seg_form;               /* CLOWNRESAMPLER_AMD_SEG_FORM: diagnostic instance of k_seg (crhip_seg_launch.debug_form) */
 	int seg_tile;               /* CLOWNRESAMPLER_AMD_SEG_TILE: k_seg's frames per lane and tile (a multiple of 16; unset: the rule) */
 	int seg_xcd_run;            /* CLOWNRESAMPLER_AMD_SEG_XCD_RUN: k_seg's consecutive tiles per XCD and round (a multiple of 4; 0: one by one; unset: CR_SEG_XCD_RUN) */
+	size_t pageable_piece;      /* CLOWNRESAMPLER_AMD_PAGEABLE_PIECE: bytes per copy from / to pageable memory (0: the variable asked for more than CR_PAGEABLE_PIECE - refused) */
 	int brief_half_tiles;       /* CLOWNRESAMPLER_AMD_BRIEF_HALF_TILES: k_up launches of fewer half wave-tiles per wave take the plan's other kernel (0: none do; unset: per instance) */
 } g_env;
 static pthread_once_t g_env_once = PTHREAD_ONCE_INIT;
@@ -449,6 +452,15 @@ static void load_env(void)
 	g_env.rotate_min_gain = (e != NULL && *e != '\0') ? atof(e) : -1.0;   /* (negative: unset - the rule's own thresholds, which differ for mono) */
 	e = getenv("CLOWNRESAMPLER_AMD_BRIEF_HALF_TILES");
 	g_env.brief_half_tiles = (e != NULL && *e != '\0' && atoi(e) >= 0) ? atoi(e) : -1;
+	e = getenv("CLOWNRESAMPLER_AMD_PAGEABLE_PIECE");
+	g_env.pageable_piece = CR_PAGEABLE_PIECE;
+	if (e != NULL && *e != '\0')
+	{
+		char *end = NULL;
+		const unsigned long long piece = strtoull(e, &end, 10);
+
+		g_env.pageable_piece = (*end == '\0' && *e >= '0' && *e <= '9' && piece <= CR_PAGEABLE_PIECE) ? (size_t)piece : 0;
+	}
 	g_env.loaded = 1;
 }
 
@@ -479,7 +491,8 @@ int ClownResamplerAMD_IsUsable(void)
 	int count = 0;
 	const int device = current_device();
 
-	if (crhip_device_count(&count) != 0 || count <= 0 || device < 0 || device >= count)
+	env_ready();
+	if (g_env.pageable_piece == 0 || crhip_device_count(&count) != 0 || count <= 0 || device < 0 || device >= count)
 		return 0;
 	if (crhip_get_device_info(device, &info) != 0)
 		return 0;
@@ -529,20 +542,13 @@ static int host_free(void *pointer)
    resource" above 1 MiB, "... Using Staging resource" up to it).  Every abort of a GPU test run that could be placed - three, rounds 5 and 6 -
    was a GPU page fault at an address inside the process's brk heap, reported while the main thread sat in such a copy (a 1.1-1.2 MB
    tensor.cpu() of the test), none of this library's launches having been given a host address (the flight recorder above).  What inside the
-   runtime or the kernel driver goes wrong has not been established (HISTORY.md, round 6); what this library can do is keep ITS copies of a
+   runtime or the kernel driver goes wrong has not been established; what this library can do is keep ITS copies of a
    client's pageable memory off that path: pieces the runtime stages through its own pinned buffers.  CLOWNRESAMPLER_AMD_PAGEABLE_PIECE in the
-   environment (bytes; 0: whole copies, the behaviour of rounds 1-5) is the A/B hook. */
-#define CR_PAGEABLE_PIECE ((size_t)1 << 20)
+   environment makes the pieces smaller; a value that would put a copy back on that path - 0 or more than 1 MiB - is refused with
+   every call that needs the device (ensure_ctx_locked), as long as the fault has no explanation. */
 static size_t pageable_piece(void)
 {
-	static size_t piece = (size_t)-1;
-
-	if (piece == (size_t)-1)
-	{
-		const char *e = getenv("CLOWNRESAMPLER_AMD_PAGEABLE_PIECE");
-		piece = (e != NULL && *e != '\0') ? (size_t)strtoull(e, NULL, 10) : CR_PAGEABLE_PIECE;
-	}
-	return piece;
+	return g_env.pageable_piece != 0 ? g_env.pageable_piece : CR_PAGEABLE_PIECE;
 }
 
 static int copy_pageable_h2d(void *device_destination, const void *host_source, size_t bytes, void *stream)
@@ -550,8 +556,6 @@ static int copy_pageable_h2d(void *device_destination, const void *host_source, 
 	const size_t piece = pageable_piece();
 	size_t at = 0;
 
-	if (piece == 0 || bytes <= piece)
-		return crhip_memcpy_h2d(device_destination, host_source, bytes, stream);
 	while (at < bytes)
 	{
 		const size_t n = bytes - at < piece ? bytes - at : piece;
@@ -569,8 +573,6 @@ static int copy_pageable_d2h(void *host_destination, const void *device_source, 
 	const size_t piece = pageable_piece();
 	size_t at = 0;
 
-	if (piece == 0 || bytes <= piece)
-		return crhip_memcpy_d2h(host_destination, device_source, bytes, stream);
 	while (at < bytes)
 	{
 		const size_t n = bytes - at < piece ? bytes - at : piece;
@@ -773,6 +775,12 @@ static cr_device_ctx *ensure_ctx_locked(int ordinal)
 		return cr_check_hip(crhip_set_device(ordinal), "hipSetDevice") == 0 ? g_ctx[ordinal] : NULL;
 
 	env_ready();
+	if (g_env.pageable_piece == 0)
+	{
+		cr_fail(CLOWNRESAMPLER_AMD_ERROR_ARGUMENT, "CLOWNRESAMPLER_AMD_PAGEABLE_PIECE must be 1 ... %lu bytes: larger copies of pageable memory are page-locked in place by "
+		        "the HIP runtime, a path with an unexplained GPU page fault on record", (unsigned long)CR_PAGEABLE_PIECE);
+		return NULL;
+	}
 	e = crhip_device_count(&count);
 
 	if (e != 0 || count <= 0)

@@ -175,11 +175,32 @@ int crhip_host_alias(const void *host, size_t bytes, void **device_alias)
 	return 1;   /* pageable: the staged path */
 }
 
+/* for the tests: the largest single copy between "device" and host memory since the last call, and how many copies there were */
+static size_t g_copy_largest;
+static unsigned long long g_copies;
+
+static void copy_seen(size_t bytes)
+{
+	size_t largest = __atomic_load_n(&g_copy_largest, __ATOMIC_RELAXED);
+
+	__atomic_fetch_add(&g_copies, 1ull, __ATOMIC_RELAXED);
+	while (bytes > largest && !__atomic_compare_exchange_n(&g_copy_largest, &largest, bytes, 0, __ATOMIC_RELAXED, __ATOMIC_RELAXED))
+		;
+}
+
+size_t crhip_fake_largest_copy(unsigned long long *copies)
+{
+	if (copies != NULL)
+		*copies = __atomic_exchange_n(&g_copies, 0ull, __ATOMIC_RELAXED);
+	return __atomic_exchange_n(&g_copy_largest, 0, __ATOMIC_RELAXED);
+}
+
 int crhip_memcpy_h2d(void *dst, const void *src, size_t bytes, void *stream)
 {
 	(void)stream;
 	if (injected(FAKE_FAIL_COPY))
 		return FAKE_ERROR_INJECTED;
+	copy_seen(bytes);
 	memcpy(dst, src, bytes);
 	return 0;
 }
@@ -189,6 +210,7 @@ int crhip_memcpy_d2h(void *dst, const void *src, size_t bytes, void *stream)
 	(void)stream;
 	if (injected(FAKE_FAIL_COPY))
 		return FAKE_ERROR_INJECTED;
+	copy_seen(bytes);
 	memcpy(dst, src, bytes);
 	return 0;
 }

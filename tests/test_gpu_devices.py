@@ -374,21 +374,23 @@ print("COPIES-OK")
 """
 
 
-def test_pageable_copies_stay_off_the_runtimes_pinned_path():
-    """Round 6's regression test: every abort of a GPU test run that could be placed was a GPU page fault at a HEAP address
+@pytest.mark.parametrize("piece", [
+    "1048576",
+    pytest.param("0", marks=pytest.mark.skip(reason="whole copies take the runtime's pinned-in-place path, where every placed GPU page fault of this suite happened; the cause "
+                                                    "is not known, and the library refuses the setting (tests/test_hostshim.py::test_pageable_copies_leave_in_pieces)"))])
+def test_pageable_copies_stay_off_the_runtimes_pinned_path(piece):
+    """Every abort of a GPU test run that could be placed was a GPU page fault at a HEAP address
     during a copy of more than 1 MiB between the device and pageable memory, which the runtime serves by page-locking the host range in place
     ("HSA Copy Using Pinned resource" in its own log).  The library's copies of a client's pageable memory - the staged host-pointer entry
-    point, CopyToDevice / CopyFromDevice - now leave in 1 MiB pieces, which the runtime stages ("... Using Staging resource"): with the
-    runtime's defaults in force, not ONE pinned copy between the markers; with CLOWNRESAMPLER_AMD_PAGEABLE_PIECE=0 (whole copies, the library of
-    rounds 1-5) the same calls make them - so the check can see what it checks."""
+    point, CopyToDevice / CopyFromDevice - leave in 1 MiB pieces, which the runtime stages ("... Using Staging resource"): with the
+    runtime's defaults in force, not ONE pinned copy between the markers.  That the pieces are what the library makes of a larger copy is
+    shown on the CPU, by the sizes of the copies (tests/test_hostshim.py)."""
     code = _COPY_PATH_SNIPPET % {"root": ROOT, "tests": os.path.join(ROOT, "tests")}
-    counts = {}
-    for piece in ("1048576", "0"):
-        env = dict(os.environ, AMD_LOG_LEVEL="4", CLOWNRESAMPLER_AMD_PAGEABLE_PIECE=piece, GPU_PINNED_MIN_XFER_SIZE="1")   # (1 MiB: the runtime's default)
-        r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600, env=env)
-        assert r.returncode == 0 and "COPIES-OK" in r.stdout, (r.stdout[-1000:], r.stderr[-2000:])
-        log = r.stderr.split("=====BEGIN", 1)[1].split("=====END", 1)[0]
-        counts[piece] = (log.count("Using Pinned resource"), log.count("Using Staging resource"))
-    if counts["0"][0] == 0:
-        pytest.skip("this runtime's log does not name its pinned copies (%r): nothing to hold the library against" % (counts,))
-    assert counts["1048576"][0] == 0 and counts["1048576"][1] > 0, counts
+    env = dict(os.environ, AMD_LOG_LEVEL="4", CLOWNRESAMPLER_AMD_PAGEABLE_PIECE=piece, GPU_PINNED_MIN_XFER_SIZE="1")   # (1 MiB: the runtime's default)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600, env=env)
+    assert r.returncode == 0 and "COPIES-OK" in r.stdout, (r.stdout[-1000:], r.stderr[-2000:])
+    log = r.stderr.split("=====BEGIN", 1)[1].split("=====END", 1)[0]
+    pinned, staged = log.count("Using Pinned resource"), log.count("Using Staging resource")
+    if pinned + staged == 0:
+        pytest.skip("this runtime's log does not name the path of its copies: nothing to hold the library against")
+    assert pinned == 0 and staged > 0, (pinned, staged)

@@ -134,3 +134,56 @@ def test_c_driver_with_the_real_instance_tables_under_sanitizers(instance_librar
     assert "ERROR: AddressSanitizer" not in r.stderr and "runtime error" not in r.stderr and "LeakSanitizer" not in r.stderr, r.stderr[-4000:]
     r = _run(targets[2], {"TSAN_OPTIONS": "halt_on_error=0:exitcode=66"}, 1200)
     assert "WARNING: ThreadSanitizer" not in r.stderr, r.stderr[-6000:]
+
+
+_PIECES_SNIPPET = r"""
+import ctypes as C, os, sys
+import numpy as np
+import clownresampler_amd as cr
+import _checkers as ck, _product
+piece = os.environ.get("CLOWNRESAMPLER_AMD_PAGEABLE_PIECE")
+lib = C.CDLL(os.environ["CLOWNRESAMPLER_AMD_LIBRARY"])
+lib.crhip_fake_largest_copy.restype = C.c_size_t
+copies = C.c_ulonglong()
+p, o = _product.Product(3), ck.oracle(3)
+ch, rates, frames = 2, (44100, 48000, 44100), 700000
+ok, st = p.low_init(ch, *rates); ok, ost = o.low_init(ch, *rates)
+padded = ck.pad_frames(ck.noise_pcm(frames * ch, 11), ch, 3)
+before = st.astuple()
+try:
+    got, left, ran_out = p.api.LowLevel_ResampleBulk(st.raw, p.pre, padded, frames)
+    d = p.api.DeviceAlloc(padded.nbytes)
+    p.api.CopyToDevice(d, padded)
+    back = np.empty_like(padded)
+    p.api.CopyFromDevice(back, d)
+    p.api.DeviceFree(d)
+except cr.ClownResamplerError as e:
+    assert "CLOWNRESAMPLER_AMD_PAGEABLE_PIECE" in str(e) and st.astuple() == before
+    assert lib.crhip_fake_largest_copy(C.byref(copies)) == 0 and copies.value == 0
+    assert p.api.IsUsable() == 0
+    print("REFUSED")
+else:
+    assert left == 0 and np.array_equal(got, o.low_resample_i32(ost, padded, frames)[0]) and np.array_equal(back, padded)
+    print("LARGEST", lib.crhip_fake_largest_copy(C.byref(copies)), copies.value)
+"""
+
+
+@pytest.mark.parametrize("piece, largest", [(None, 1 << 20), ("1048576", 1 << 20), ("65536", 65536), ("100001", 100001),
+                                            ("0", None), ("1048577", None), ("-1", None), ("1M", None), ("18446744073709551617", None)])
+def test_pageable_copies_leave_in_pieces(drivers, piece, largest):
+    """Every copy between the device and pageable memory is at most 1 MiB - or CLOWNRESAMPLER_AMD_PAGEABLE_PIECE, which can only make the pieces
+    smaller: larger copies are page-locked in place by the HIP runtime, the path all placed GPU page faults of this library's test runs
+    were on.  A value that would bring them back (0, more than 1 MiB, no number) is refused with the call, nothing copied, no state moved.
+    Shown here, on the fake seam, by the sizes of the copies; on the GPU only the default is ever run."""
+    env = dict(os.environ, CLOWNRESAMPLER_AMD_LIBRARY=os.path.join(BUILD, "libcr_hostshim.so"), CRA_FAKE_DEVICES="1", PYTHONPATH=ROOT + os.pathsep + os.path.join(ROOT, "tests"))
+    env.pop("CLOWNRESAMPLER_AMD_PAGEABLE_PIECE", None)
+    if piece is not None:
+        env["CLOWNRESAMPLER_AMD_PAGEABLE_PIECE"] = piece
+    r = subprocess.run(["python3", "-c", _PIECES_SNIPPET], capture_output=True, text=True, timeout=300, env=env)
+    assert r.returncode == 0, (r.stdout[-1000:], r.stderr[-3000:])
+    word, *rest = r.stdout.split()
+    if largest is None:
+        assert word == "REFUSED", r.stdout
+    else:
+        total = 2 * 2 * 700000 + 2 * 4 * 761904   # the input and the output of the bulk call, at the least
+        assert word == "LARGEST" and int(rest[0]) == largest and int(rest[1]) >= total // largest, r.stdout
