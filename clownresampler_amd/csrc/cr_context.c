@@ -2692,11 +2692,11 @@ static void workspace_release(cr_device_ctx *ctx)
 }
 
 /* ---- pipelined host path ----
-   hipMemcpyAsync on pageable memory does not return before the copy is done (measured: tools/microbench/pinbench.hip), so
+   hipMemcpyAsync on pageable memory does not return before the copy is done (measured: profiles/r01_pinbench.log), so
    one host thread can never have an upload and a download in flight together.  For calls of more than one batch a
    second thread therefore does the downloads: while it copies batch b's output (and waits for b's kernel before that),
    the calling thread uploads batch b + 1 into another staging set and launches it.  PCIe is full duplex: the upload
-   hides behind the download (pinbench: 4.5-4.8 ms instead of 6.0 ms for the 106 MB + 230 MB of cfg 2; this path:
+   hides behind the download (the same log: 4.5-4.8 ms instead of 6.0 ms for the 106 MB + 230 MB of cfg 2; this path:
    6.3 -> 5.0 ms).  Three staging sets: with two, the upload of batch b + 2 had to wait for download b and then ran
    side by side with download b + 1, slowing both, and the download thread idled in between (5.6 ms). */
 typedef struct cr_download

@@ -52,7 +52,6 @@ def child(mode):
         pin_in.numpy()[:] = pcm
         pinned = [once(pin_in.numpy(), pin_out.numpy()) for _ in range(5)]
         same = bool(np.array_equal(pin_out.numpy()[: n_out * ch], out[: n_out * ch]))
-        # a registered range that starts in the middle of a page-locked block (hipHostRegister'ed malloc memory)
         res[name] = {"pageable_ms": min(pageable[1:]), "pinned_ms": min(pinned[1:]), "pinned_first_ms": pinned[0], "same": same,
                      "MB": (pcm.nbytes + n_out * ch * 4) / 1e6}
         del pin_in, pin_out
