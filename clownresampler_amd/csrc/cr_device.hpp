@@ -1168,35 +1168,35 @@ __device__ __forceinline__ void one_frame(const crhip_poly_launch &a, const int 
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Tickets.  draw_ticket returns the counter's value before the increment, once per WAVE (a scalar instruction: every lane of
-// the calling wave sees the same value; call it from wave-uniform control flow only).  It is s_atomic_add: the value comes
-// back through lgkmcnt into an SGPR and the wait for it, here, is this wave's own round trip to the L2 and nothing else.  The
-// obvious form - lane 0 does a vector atomic - returns through vmcnt into a VGPR, and hipcc waits for that register with
-// vmcnt(0) long before it is used (it rewrites a single-lane atomic into the wave-aggregated form, whose readfirstlane needs
-// the value on the spot; and with that turned off it still flushes at the head of any loop that reads the register): the
-// wave's outstanding stores and LDS-DMA are drained once per ticket.  tools/microbench/satomic.hip checks that scalar atomics
-// exist on gfx950 and hand out dense, unique values next to vector atomics on the same word.
+// Tickets, once per WAVE, from wave-uniform control flow with every lane active.  draw_ticket_begin: lane 0 adds 1 to the counter and
+// the value before the addition travels into a VGPR of the caller's; draw_ticket_end: the wave has it, in a scalar.
+// The atomic is a returning VECTOR instruction: it counts in vmcnt, with the wave's loads, LDS-DMA and stores, in issue order.  hipcc knows
+// of the pending register and waits at its first use - the end of the draw - until no more VMEM instructions are outstanding than it can
+// COUNT behind the draw.  So a draw goes in FRONT of the tile's stores, next to the DMA, and is ended behind the tile's own counted wait
+// (which has then covered it) and in straight-line code: behind a loop of stores hipcc counts none of them and drains them all.
+// That is why k_poly ends the draw in each of its tile sizes' arms, and why k_up2 and k_wave2 deal all but their last rounds statically.
+// `got` is set once, outside the loop, and afterwards by draws alone: the flow graph has paths on which a draw is never ended (no wave
+// takes them), and on its next write by anything but another VMEM instruction hipcc would drain everything in front of it.
+// The address goes through a VGPR that hipcc knows nothing about: for an address it can prove uniform it rewrites even a single-lane
+// atomic into the wave-aggregated form, whose readfirstlane waits for the value on the spot.
 // ---------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ unsigned draw_ticket(unsigned *counter)
+__device__ __forceinline__ void draw_ticket_begin(unsigned *counter, unsigned &got)
 {
-	unsigned got = 1u;
-	asm volatile("s_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(got) : "s"(counter) : "memory");
-	return got;
-}
-
-// The same in two halves, for a caller that has a wait of its own to put in between (the round trip then runs under it).  The
-// SGPR is in flight between the two: NOTHING but the caller's own inline-assembly waits may stand between them - hipcc knows
-// nothing of the pending write and would read the register early if it had a reason to touch it.
-__device__ __forceinline__ unsigned draw_ticket_begin(unsigned *counter)
-{
-	unsigned got = 1u;
-	asm volatile("s_atomic_add %0, %1, 0x0 glc" : "+s"(got) : "s"(counter) : "memory");
-	return got;
+	typedef __attribute__((address_space(1))) unsigned global_unsigned;
+	typedef __attribute__((address_space(1))) unsigned char global_byte;
+	if ((threadIdx.x & 63u) == 0)
+	{
+		// (volatile: made here and dead behind the atomic - hoisted out of the tile loop they cost k_poly two registers of its 64)
+		unsigned offset = 0, one = 1;
+		asm volatile("" : "+v"(offset), "+v"(one));
+		got = __hip_atomic_fetch_add((global_unsigned *)((global_byte *)counter + offset), one, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+	}
 }
 __device__ __forceinline__ unsigned draw_ticket_end(unsigned got)
 {
-	asm volatile("s_waitcnt lgkmcnt(0)" : "+s"(got) : : "memory");
-	return got;
+	// (volatile and a memory barrier to hipcc: its own wait for the register stands here, behind the caller's counted wait)
+	asm volatile("" : "+v"(got) : : "memory");
+	return (unsigned)__builtin_amdgcn_readfirstlane((int)got);
 }
 
 // ---------------------------------------------------------------------------------------------------------

@@ -119,8 +119,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_int(const crhip_int_launch a)
 
 	// Wave-tiles are TICKETS where the launch brings counters (long launches): the first by global wave number, every further one
 	// from 32 global counter lanes, as in k_up2 - the XCDs of one chip hold different clocks under this kind of load (1.9-2.1 GHz),
-	// and with equal static shares a launch lasts as long as its slowest XCD.  A ticket is a scalar atomic (draw_ticket: through
-	// lgkmcnt, not through the vmcnt the stores and the DMA share).  The last wave of the last workgroup zeroes the block again.
+	// and with equal static shares a launch lasts as long as its slowest XCD.  The last wave of the last workgroup zeroes the block again.
 	// A ticket is worth G consecutive tiles: 8,192 waves drawing 75,000 single-tile tickets from 32 counters were bound by the atomics
 	// (mono 6:1: 66.5 us static, 71.9 us ticketed; profiles/r03_kint_tickets.log).  The unit of scheduling is the GROUP below.
 	const bool ticketed = a.d_tickets != nullptr;
@@ -132,7 +131,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_int(const crhip_int_launch a)
 	const unsigned lane_waves = (unsigned)((global_waves - lane_id + LANES - 1u) / LANES);
 	unsigned *lane_counter = a.d_tickets + lane_id * 32u;
 	auto resolve = [&](unsigned got) -> uint64_t {
-		const uint64_t k = (uint64_t)lane_waves + (unsigned)__builtin_amdgcn_readfirstlane((int)got);
+		const uint64_t k = (uint64_t)lane_waves + draw_ticket_end(got);
 		return k < lane_tiles ? lane_id + (uint64_t)LANES * k : ~0ull;
 	};
 	unsigned *waves_done = reinterpret_cast<unsigned *>(smem + WAVES * (WIN + STAGE));
@@ -205,13 +204,16 @@ __global__ __launch_bounds__(WAVES * 64) void k_int(const crhip_int_launch a)
 		}
 	};
 
-	// `next` is known a tile ahead: its ticket is drawn at the END of the previous tile, the atomic's round trip running under the
-	// wait for that tile's DMA (a draw that is waited for on the spot cost the short mono tiles 7 %: profiles/r03_kint_tickets.log)
+	// `next` is known a tile ahead: its ticket is drawn in the previous tile, the atomic's round trip running under that
+	// tile's stores and the wait for its DMA (a draw that is waited for on the spot cost the short mono tiles 7 %: profiles/r03_kint_tickets.log)
 	// (`next_group`: the group after the one in progress; within a group the tiles follow each other)
 	uint64_t tile = global_wave * G;
 	unsigned in_group = 1;
 	unsigned lost = fetch(tile);
-	uint64_t next_group = ticketed ? resolve(draw_ticket(lane_counter)) : (global_wave + global_waves < n_groups ? global_wave + global_waves : ~0ull);
+	unsigned ticket = 0;
+	if (ticketed)
+		draw_ticket_begin(lane_counter, ticket);
+	uint64_t next_group = ticketed ? resolve(ticket) : (global_wave + global_waves < n_groups ? global_wave + global_waves : ~0ull);
 	uint64_t next = (G > 1u && tile + 1u < n_tiles) ? tile + 1u : (next_group != ~0ull ? next_group * G : ~0ull);
 	if (G > 1u && tile + 1u >= n_tiles)
 		in_group = G;   // (the stream's last group is a short one)
@@ -432,6 +434,11 @@ __global__ __launch_bounds__(WAVES * 64) void k_int(const crhip_int_launch a)
 		__builtin_amdgcn_wave_barrier();
 		__builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 
+		// where `next` enters a new group: the ticket for the group after that one, in front of this tile's stores
+		const bool entering = in_group == G;       // `next` is the first tile of next_group
+		if (have_next && entering && ticketed)
+			draw_ticket_begin(lane_counter, ticket);
+
 		// copy-out: the tile's n frames are contiguous in the output; wave-uniform base, one lane offset: 16 bytes per lane (dword
 		// alignment is all gfx950 asks of global_store_dwordx4), then the tail by dwords and - int16 mono - one last sample
 		unsigned stores = 0;
@@ -484,24 +491,13 @@ __global__ __launch_bounds__(WAVES * 64) void k_int(const crhip_int_launch a)
 
 		if (!have_next)
 			break;
-		// the DMA was issued before this tile's stores and vmcnt retires in order: the stores stay in flight.  The ticket for the
-		// tile after the next one travels meanwhile (nothing but our own waits between the two halves of the draw).
-		// (`next` was the tile being fetched; what comes after it: the next tile of its group, or the first of the following group -
-		// whose own successor is drawn now, when the wave enters a new group)
-		const bool entering = in_group == G;       // `next` is the first tile of next_group
-		if (entering && ticketed)
-		{
-			unsigned ticket = draw_ticket_begin(lane_counter);
-			wait_vmcnt_at_most(stores);
-			ticket = draw_ticket_end(ticket);
-			next_group = resolve(ticket);
-		}
-		else
-		{
-			wait_vmcnt_at_most(stores);
-			if (entering)
-				next_group = (next / G) + global_waves < n_groups ? (next / G) + global_waves : ~0ull;
-		}
+		// the DMA and the draw were issued before this tile's stores and vmcnt retires in order: the stores stay in flight - but for
+		// the last tile of a group, whose ticket hipcc waits for until no more stores are out than it can count (none: they are
+		// issued from loops).  Once per G tiles.
+		// (`next` was the tile being fetched; what comes after it: the next tile of its group, or the first of the following group)
+		wait_vmcnt_at_most(stores);
+		if (entering)
+			next_group = ticketed ? resolve(ticket) : (next / G) + global_waves < n_groups ? (next / G) + global_waves : ~0ull;
 		tile = next;
 		in_group = entering ? 1u : in_group + 1u;
 		next = (in_group < G && tile + 1u < n_tiles) ? tile + 1u : (next_group != ~0ull ? next_group * G : ~0ull);

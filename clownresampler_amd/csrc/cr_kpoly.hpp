@@ -36,8 +36,17 @@ namespace
 //           the two halves of the workgroup into the two halves of the DMA buffer, interleaved into a stereo tile by an LDS -> LDS
 //           pass (four frames per thread: four funnel shifts, four byte permutes, one 16-byte write), and the results leave as two 4-byte stores H frames
 //           apart.  crhip_poly_launch.dual* carry H, how many second frames exist, and the input offset; n_out counts pairs.
+// waves per SIMD asked of the register allocator: what the workgroup needs anyway, but for a few shapes that would take 65 VGPRs - one
+// over two workgroups per CU - and fit into 64 when told to: six channels per lane with 5 slots or (11 channels) run-time ones, and the
+// int16 output of three and four channels with 6 slots
+template <int CH, int TT, int NTHREADS, int ASM, int OUT16, int SPLIT, int PH, int PADT>
+constexpr unsigned poly_waves_per_simd()
+{
+	return (CH == 6 && TT == 0 && SPLIT == 2 && PH == 1 && PADT == 0) || (CH == 6 && TT == 5 && SPLIT == 1 && ASM == 1) || ((CH == 3 || CH == 4) && TT == 6 && OUT16 && SPLIT == 1 && ASM == 3) ? 8u : NTHREADS / 256u;
+}
+
 template <int CH, int TT, int MODE, int NORM, int NTHREADS, int NV, int ASM, int U, int SWZ, int ABL = 0, int OUT16 = 0, int NT = 0, int SPLIT = 1, int PH = 0, int DUAL = 0, int PADT = 0>
-__global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR_BUDGET))) void k_poly(const crhip_poly_launch a)
+__global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR_BUDGET), amdgpu_waves_per_eu(poly_waves_per_simd<CH, TT, NTHREADS, ASM, OUT16, SPLIT, PH, PADT>()))) void k_poly(const crhip_poly_launch a)
 {
 	static_assert(!DUAL || (CH == 2 && SPLIT == 1 && PH == 0 && OUT16 == 0 && TT > 0 && ABL == 0 && (NTHREADS / 2) % 64 == 0), "dual mono: a stereo instance, int32 output");
 	constexpr unsigned CHT = CH * SPLIT - PH;             // channels of a frame
@@ -188,12 +197,12 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 	// (Helping other sequences out once the own one is exhausted was tried: deciding where to draw needs the counter's
 	// value NOW, and a dependent load at the top of every tile stalls wave 0 - and with it the workgroup - for a memory
 	// round trip per tile: 148 us instead of 64.  The draw below has no consumer until the end of the tile.)
-	// The draw is a scalar atomic (draw_ticket, cr_device.hpp), made by wave 0 alone (wave-uniform branch).  As a vector atomic
-	// of thread 0 it cost wave 0 a vmcnt(0) per tile - every store of the previous tile and the DMA just issued - which was the
-	// "issuing the next tile's DMA" share of a tile in the stamped diagnostic instance (42-44 % of wave 0's cycles, the other
-	// waves waiting for it at the barrier).
-	auto draw = [&]() -> unsigned {
-		const uint64_t k = (uint64_t)lane_groups + draw_ticket(lane_counter);
+	// Wave 0 alone draws (wave-uniform branch): behind the next tile's DMA and in front of this tile's stores, so the tile's counted
+	// wait covers it (cr_device.hpp, "Tickets").  Ended anywhere hipcc cannot count the stores, the draw costs wave 0 a vmcnt(0)
+	// per tile - 42-44 % of its cycles in the stamped diagnostic instance, the other waves waiting for it at the barrier.
+	// The ticket goes to every wave through the mailbox as it came.
+	auto resolve = [&](unsigned ticket) -> unsigned {
+		const uint64_t k = (uint64_t)lane_groups + ticket;
 		return k < lane_tiles ? (unsigned)(lane_id + LANES * k) : 0xFFFFFFFFu;
 	};
 	const bool wave0 = __builtin_amdgcn_readfirstlane((int)(tid >> 6)) == 0;
@@ -218,11 +227,12 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 	// a.dynamic_tiles == 0: plain round-robin (tile + gridDim.x), no tickets - for configurations whose tiles are so
 	// small that a ticket and a mailbox hand-over per tile cost more than the imbalance they remove (8-channel frames)
 	const bool dynamic = a.dynamic_tiles != 0;
+	unsigned ticket = 0;
 	if (dynamic && wave0)
 	{
-		const unsigned first_ticket = draw();
+		draw_ticket_begin(lane_counter, ticket);
 		if (tid == 0)
-			mailbox[0] = first_ticket;
+			mailbox[0] = ticket;
 	}
 	// stage the polyphase rows once per workgroup (L2-resident after the first workgroups) - AFTER the first tile's DMA and
 	// the first ticket are on their way, so that the three round trips of a workgroup's start overlap
@@ -292,7 +302,7 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 	}
 	asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
 	__syncthreads();   // rows staged (plain stores to LDS), first tile landed and first ticket posted, for every wave
-	uint64_t next_index = dynamic ? __builtin_amdgcn_readfirstlane(mailbox[0]) : tile_index + gridDim.x;   // wave-uniform
+	uint64_t next_index = dynamic ? resolve(__builtin_amdgcn_readfirstlane(mailbox[0])) : tile_index + gridDim.x;   // wave-uniform
 
 	// diagnostic instance (ABL == 6) only: where a tile's cycles go, summed over the tiles of this workgroup as seen by
 	// wave 0 - [0] issuing the next tile's DMA + ticket, [1] arithmetic + stores, [2] waiting for the DMA (vmcnt),
@@ -326,7 +336,6 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 		const bool more = next_index < n_tiles;
 		const uint64_t jn = next_index * NT64;
 		unsigned n_next = 0, shift_next = 0;
-		unsigned ticket = 0;
 
 		if constexpr (DUAL)
 		{
@@ -400,7 +409,7 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 			n_next = (unsigned)((a.n_out - jn < NT64) ? (a.n_out - jn) : NT64);
 			shift_next = fetch(jn, n_next, (DUAL || PADL) ? tiles : tiles + ((it + 1u) & 1u) * TILE_BYTES);
 			if (dynamic && wave0)
-				ticket = draw();   // for the tile after the next one; posted below, just before the barrier
+				draw_ticket_begin(lane_counter, ticket);   // for the tile after the next one; ended in this tile's arm, posted just before the barrier
 		}
 		mark(0);
 
@@ -512,6 +521,8 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 			}
 		};
 
+		unsigned drawn = 0;   // the ticket, for wave 0 (nobody looks at it where none was drawn)
+
 		// Full tiles of 4, 3, 2 or 1 groups as straight-line code (see the vmcnt note above).  Specialised instances
 		// (TT > 0) run the frames of a tile as a software pipeline: the LDS reads of frame i+1 are issued before the
 		// arithmetic of frame i.
@@ -566,6 +577,7 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 				asm volatile("s_waitcnt vmcnt(%0)" ::"i"(G * STORES_PER_GROUP) : "memory");
 			else
 				asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+			drawn = draw_ticket_end(ticket);
 			mark(2);
 		};
 
@@ -598,6 +610,7 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 					store_ints<CH, NT>(out_tile + (size_t)jl * CH, outv);
 			}
 			asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+			drawn = draw_ticket_end(ticket);
 		}
 
 		if constexpr (ABL == 6)
@@ -629,7 +642,7 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 		// every wave's share of the next tile has landed once every wave is past its wait; the mailbox has two slots,
 		// used alternately, so that a slot is never rewritten before every wave has read it
 		if (dynamic && tid == 0)
-			mailbox[(it + 1u) & 1u] = ticket;
+			mailbox[(it + 1u) & 1u] = drawn;
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 		__builtin_amdgcn_s_barrier();
 		mark(3);
@@ -637,7 +650,7 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 		jt = jn;
 		n = n_next;
 		shift = shift_next;
-		next_index = dynamic ? __builtin_amdgcn_readfirstlane(mailbox[(it + 1u) & 1u]) : tile_index + gridDim.x;
+		next_index = dynamic ? resolve(__builtin_amdgcn_readfirstlane(mailbox[(it + 1u) & 1u])) : tile_index + gridDim.x;
 	}
 }
 

@@ -112,7 +112,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 	const unsigned lane_waves = (unsigned)((global_waves - lane_id + LANES - 1u) / LANES);
 	unsigned *lane_counter = a.d_tickets + lane_id * 32u;
 	auto draw_resolve = [&](unsigned got) -> uint64_t {
-		const uint64_t k = (uint64_t)lane_waves + (unsigned)__builtin_amdgcn_readfirstlane((int)got);
+		const uint64_t k = (uint64_t)lane_waves + got;
 		return k < lane_tiles ? tile_of(k) : ~0ull;
 	};
 	auto retire = [&]() {
@@ -183,16 +183,12 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 		return;
 	}
 	uint64_t tile = tile_of(global_wave / LANES);
+	unsigned ticket = 0;
 
 	for (;;)
 	{
-		// the ticket for the tile after this one: its round trip runs under the tile
-		// (the counter's address rebuilt from scalar halves: with this kernel's scalar register pressure hipcc otherwise parks the pointer in a VGPR pair,
-		// which the scalar atomic cannot take)
-		const uint64_t counter_bits = reinterpret_cast<uint64_t>(lane_counter);
-		unsigned *const counter = reinterpret_cast<unsigned *>(((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(counter_bits >> 32)) << 32)
-		                                                       | (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)counter_bits));
-		const unsigned ticket = draw_ticket_begin(counter);
+		// the ticket for the tile after this one: its round trip runs under that of the tile's first window
+		draw_ticket_begin(lane_counter, ticket);
 		mark(-1);
 
 		// ---- where the tile is ----
@@ -242,6 +238,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 		top_up(0);
 		// (the previous tile's last stores are older than these requests: all of it has to land - once per tile)
 		asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+		const unsigned drawn = draw_ticket_end(ticket);
 		f32x2 P[TT][2];   // slot s of rotation R is P[(s + R) % TT]
 #pragma unroll
 		for (int s = 0; s < TT; ++s)
@@ -474,7 +471,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 
 		asm volatile("s_setreg_b32 hwreg(HW_REG_MODE, 0, 2), %0" ::"s"(fp_mode));
 
-		const uint64_t next = draw_resolve(draw_ticket_end(ticket));
+		const uint64_t next = draw_resolve(drawn);
 		if (next == ~0ull)
 			break;
 		tile = next;

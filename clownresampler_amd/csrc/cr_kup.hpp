@@ -581,25 +581,29 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 	}
 	__syncthreads();
 
-	// Wave-tiles are TICKETS, as in k_wave: the first by global wave number, every further one from 32 global counter lanes.
-	// The XCDs of one chip do not run this kernel at one speed - under sustained load their clocks sit between 1.9 and 2.1 GHz,
-	// and with equal static shares the launch lasted as long as the slowest XCD (end times 143 .. 159 us,
-	// profiles/r02_kup2_sweep.log) - so whoever is free takes the next tile.  A ticket is a scalar atomic (draw_ticket, cr_device.hpp:
-	// through lgkmcnt, not through the vmcnt the stores and the DMA share), drawn a tile ahead of its use, its round trip under the
-	// wait for the next window.
+	// Who takes which wave-tile: as in k_wave2, round-robin over the waves for all but the last two rounds, the tiles of those as
+	// TICKETS from 32 global counter lanes (a wave's first tile of the ticketed region is implicit).  The XCDs of one chip do not
+	// run this kernel at one speed - under sustained load their clocks sit between 1.9 and 2.1 GHz, and with equal static shares
+	// the launch lasted as long as the slowest XCD (end times 143 .. 159 us, profiles/r02_kup2_sweep.log) - so whoever is free takes
+	// the next tile of the tail.  A ticket is drawn a tile ahead of its use, in front of the stores; waiting for it drains that tile's
+	// (they leave from a loop: cr_device.hpp, "Tickets"), which is what the tiles in front of the tail are spared.
 	const uint64_t n_tiles = (a.n_out + WT - 1) / WT;
 	const uint64_t global_wave = (uint64_t)wave * gridDim.x + blockIdx.x;   // (a short launch spreads over the CUs, not over a CU's waves)
 	const uint64_t global_waves = (uint64_t)gridDim.x * WAVES;
+	const uint64_t rounds = n_tiles / global_waves;
+	const uint64_t static_limit = rounds > 2u ? (rounds - 2u) * global_waves : 0;   // tiles [0, static_limit) are dealt statically
+	const uint64_t region_tiles = n_tiles - static_limit;                           // the ticketed region, numbered from 0
 	const unsigned LANES = global_waves < 32u ? (unsigned)global_waves : 32u;
 	const unsigned lane_id = (unsigned)(global_wave % LANES);
-	const uint64_t lane_tiles = n_tiles > lane_id ? (n_tiles - lane_id + LANES - 1u) / LANES : 0;   // tiles of this counter's sequence
-	const unsigned lane_waves = (unsigned)((global_waves - lane_id + LANES - 1u) / LANES);          // its waves = its pre-assigned tiles
+	const uint64_t lane_tiles = region_tiles > lane_id ? (region_tiles - lane_id + LANES - 1u) / LANES : 0;   // tiles of this counter's sequence
+	const unsigned lane_waves = (unsigned)((global_waves - lane_id + LANES - 1u) / LANES);                    // its waves = its pre-assigned tiles
 	unsigned *lane_counter = a.d_tickets + lane_id * 32u;
-	auto draw_issue = [&]() -> unsigned { return draw_ticket(lane_counter); };   // (scalar, the whole wave: cr_device.hpp)
 	auto draw_resolve = [&](unsigned got) -> uint64_t {
-		const uint64_t k = (uint64_t)lane_waves + (unsigned)__builtin_amdgcn_readfirstlane((int)got);
-		return k < lane_tiles ? lane_id + (uint64_t)LANES * k : ~0ull;
+		const uint64_t k = (uint64_t)lane_waves + draw_ticket_end(got);
+		return k < lane_tiles ? static_limit + lane_id + (uint64_t)LANES * k : ~0ull;
 	};
+	// the statically known successor of a tile in front of the ticketed region
+	auto dealt = [&](uint64_t t) -> uint64_t { return t + global_waves < n_tiles ? t + global_waves : ~0ull; };
 	// a wave that has run out of tickets retires; the last wave of a workgroup reports to the global finished counter and the
 	// last workgroup zeroes the ticket block for the next launch (see k_wave)
 	auto retire = [&]() {
@@ -658,7 +662,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 	// one wave-tile: n output frames from `first`, window at `base`; returns the number of store instructions issued
 	constexpr unsigned SAFEMASK = mad_safemask<TT>();
 	static_assert(TT > 1 && SAFEMASK != 0 && (SAFEMASK & NEGMASK) == 0 && !(SAFEMASK & 1u) && !(NEGMASK & 0u), "slot classes of the instance: slot 0 ordinary, the centre slots never negative");
-	auto wave_tile = [&](uint64_t first, unsigned n, const unsigned char *base) -> unsigned {
+	// (`draw`: whether the tile draws a ticket, which then goes to `ticket`)
+	auto wave_tile = [&](uint64_t first, unsigned n, const unsigned char *base, bool draw, unsigned &ticket) -> unsigned {
 		const uint64_t pos = a.pos0 + first * (uint64_t)a.increment;
 		const unsigned frac0 = (unsigned)(pos & 0xFFFFu);
 
@@ -1011,6 +1016,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 			else
 				__builtin_amdgcn_raw_buffer_store_b32(v, out_rsrc, (int)(lane * VEC), (int)(at_vector * VEC), NT ? 2 : 0);
 		};
+		if (draw)
+			draw_ticket_begin(lane_counter, ticket);
 		unsigned stores = 0;   // wave-uniform
 		for (unsigned done = 0; done < vectors; done += 256u)
 		{
@@ -1035,14 +1042,17 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 	}
 
 	unsigned cur = 0, shift = 0;
+	unsigned ticket = 0;
 	uint64_t next;
 	{
-		const unsigned ticket = draw_issue();
+		const bool drawn = tile >= static_limit;
+		if (drawn)
+			draw_ticket_begin(lane_counter, ticket);
 		const uint64_t first = tile * WT;
 		const unsigned n = (unsigned)((a.n_out - first < WT) ? (a.n_out - first) : WT);
 		shift = fetch(first, n, my_buf);
 		asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-		next = draw_resolve(ticket);
+		next = drawn ? draw_resolve(ticket) : dealt(tile);
 	}
 	mark(-1);
 
@@ -1060,20 +1070,18 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 			const unsigned nn = (unsigned)((a.n_out - nf < WT) ? (a.n_out - nf) : WT);
 			shift_next = fetch(nf, nn, my_buf + (cur ^ 1u) * BUF);
 		}
-
-		const unsigned stores = wave_tile(first, n, my_buf + cur * BUF + shift);
+		// ... and the ticket for the tile after the next one, likewise (in front of the copy-out: a register less across the frames)
+		const bool drawn = have_next && next >= static_limit;
+		const unsigned stores = wave_tile(first, n, my_buf + cur * BUF + shift, drawn, ticket);
 
 		if (!have_next)
 			break;
-		// the ticket for the tile after the next one: its round trip runs under the wait for the next tile's window
-		unsigned ticket = draw_ticket_begin(lane_counter);
 		wait_vmcnt_at_most(stores);
-		ticket = draw_ticket_end(ticket);
-		mark(3);
 		cur ^= 1u;
 		shift = shift_next;
 		tile = next;
-		next = draw_resolve(ticket);
+		next = drawn ? draw_resolve(ticket) : dealt(tile);
+		mark(3);
 	}
 
 	retire();

@@ -72,9 +72,8 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_num_sgpr(CRHIP_SG
 	unsigned *lane_counter = a.d_tickets + lane_id * 32u;
 	// the draw is split: the atomic is issued at the start of a chunk, its result is first looked at when the last
 	// wave-tile of the chunk needs it - by then the per-wave-tile vmcnt waits have long covered it
-	auto draw_issue = [&]() -> unsigned { return draw_ticket(lane_counter); };   // (scalar, the whole wave: cr_device.hpp)
 	auto draw_resolve = [&](unsigned got) -> uint64_t {
-		const uint64_t k = (uint64_t)lane_waves + __builtin_amdgcn_readfirstlane(got);
+		const uint64_t k = (uint64_t)lane_waves + draw_ticket_end(got);
 		return k < lane_chunks ? lane_id + (uint64_t)LANES * k : ~0ull;
 	};
 	// a wave that has run out of tickets retires; the waves of a workgroup count down in LDS and only the last of them
@@ -163,7 +162,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_num_sgpr(CRHIP_SG
 	}
 
 	uint64_t chunk = global_wave;
-	unsigned parity = 0;
+	unsigned parity = 0, ticket = 0;
 	// first wave-tile of the first chunk
 	{
 		const uint64_t first = chunk * CHUNK;
@@ -176,7 +175,7 @@ __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_num_sgpr(CRHIP_SG
 
 	for (;;)
 	{
-		const unsigned ticket = draw_issue();          // one chunk ahead; resolved at the end of this chunk
+		draw_ticket_begin(lane_counter, ticket);       // one chunk ahead; resolved at the end of this chunk
 		uint64_t next_chunk = ~0ull;
 		const uint64_t chunk_first = chunk * CHUNK;
 		const bool full = chunk_first + CHUNK <= a.n_out;

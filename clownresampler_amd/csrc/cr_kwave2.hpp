@@ -120,9 +120,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_wave2(const crhip_poly_launch a)
 	// Who takes which chunk.  Chunks go round-robin over the waves (wave w: chunks w, w + waves, ...) for all but the last two
 	// rounds - no atomics, nothing to wait for - and the chunks of those last rounds are drawn as tickets, as in k_wave (32 counter
 	// lanes; a wave's first chunk of the ticketed region is implicit), so that the waves that got ahead (the XCDs differ by 10 %
-	// in clock under load) take more of the tail.  Why not tickets throughout: a returning atomic is a VMEM load into a VGPR,
-	// and hipcc waits for such a register at the head of any loop that uses it - vmcnt(0), every store of the previous chunk
-	// included - however far apart issue and use are put.  (Worth 1-4 %: profiles/r02_kwave2_trials.log.)
+	// in clock under load) take more of the tail.  Why not tickets throughout: the wait for a returning atomic drains the stores
+	// hipcc cannot count behind it (cr_device.hpp, "Tickets"), here all of the chunk's.  (Worth 1-4 %: profiles/r02_kwave2_trials.log.)
 	const uint64_t rounds = n_chunks / global_waves;
 	// (a launch of three rounds or fewer is dealt statically altogether: a draw is a memory round trip per chunk, more than the
 	// balance of so few chunks is worth)
@@ -134,9 +133,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_wave2(const crhip_poly_launch a)
 	const uint64_t lane_chunks = region_chunks > lane_id ? (region_chunks - lane_id + LANES - 1u) / LANES : 0;
 	const unsigned lane_waves = (unsigned)((global_waves - lane_id + LANES - 1u) / LANES);
 	unsigned *lane_counter = a.d_tickets + lane_id * 32u;
-	auto draw_issue = [&]() -> unsigned { return draw_ticket(lane_counter); };   // (scalar, the whole wave: cr_device.hpp)
 	auto draw_resolve = [&](unsigned got) -> uint64_t {
-		const uint64_t k = (uint64_t)lane_waves + (unsigned)__builtin_amdgcn_readfirstlane((int)got);
+		const uint64_t k = (uint64_t)lane_waves + draw_ticket_end(got);
 		return k < lane_chunks ? static_limit + lane_id + (uint64_t)LANES * k : ~0ull;
 	};
 	auto retire = [&]() {
@@ -892,9 +890,10 @@ __global__ __launch_bounds__(WAVES * 64) void k_wave2(const crhip_poly_launch a)
 		});
 	}
 	// ... and the ticketed ones (a ticket is drawn when a chunk is entered and resolved in its last tile)
+	unsigned ticket = 0;
 	while (chunk != ~0ull)
 	{
-		const unsigned ticket = draw_issue();
+		draw_ticket_begin(lane_counter, ticket);
 		chunk = run_chunk(chunk, [&]() -> uint64_t { return draw_resolve(ticket); });
 	}
 

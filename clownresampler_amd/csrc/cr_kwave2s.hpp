@@ -81,9 +81,8 @@ __global__ __launch_bounds__(1024) void k_wave2s(const crhip_poly_launch a)
 	const uint64_t lane_chunks = region_chunks > lane_id ? (region_chunks - lane_id + LANES - 1u) / LANES : 0;
 	const unsigned lane_waves = (unsigned)((global_waves - lane_id + LANES - 1u) / LANES);
 	unsigned *lane_counter = a.d_tickets + lane_id * 32u;
-	auto draw_issue = [&]() -> unsigned { return draw_ticket(lane_counter); };
 	auto draw_resolve = [&](unsigned got) -> uint64_t {
-		const uint64_t k = (uint64_t)lane_waves + (unsigned)__builtin_amdgcn_readfirstlane((int)got);
+		const uint64_t k = (uint64_t)lane_waves + draw_ticket_end(got);
 		return k < lane_chunks ? static_limit + lane_id + (uint64_t)LANES * k : ~0ull;
 	};
 	auto retire = [&]() {
@@ -368,9 +367,10 @@ __global__ __launch_bounds__(1024) void k_wave2s(const crhip_poly_launch a)
 			return next < n_chunks ? next : ~0ull;
 		});
 	}
+	unsigned ticket = 0;
 	while (chunk != ~0ull)
 	{
-		const unsigned ticket = draw_issue();
+		draw_ticket_begin(lane_counter, ticket);
 		chunk = run_chunk(chunk, [&]() -> uint64_t { return draw_resolve(ticket); });
 	}
 

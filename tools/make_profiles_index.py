@@ -27,6 +27,8 @@ for doc in ("DESIGN.md", "README.md", "INTEGRATION.md"):
 cited.pop("INDEX.md", None)   # (this file)
 missing = [n for n in cited if not os.path.exists(os.path.join(P, n))]
 WHAT = [
+    (r"vector_tickets_all_workloads\.log", "every workload of bench.py once, tickets drawn by vector atomics"),
+    (r"vector_tickets_ab\.log", "ticketed against round-robin tiles in `k_poly`, same box, three times each in turn"),
     (r"r06_bench_cfg2\.json", "the headline `bench.py` line (BASELINE configs[1], N = 1) of round 6's final build, with `roofline`, `cpu_baseline`, `parity_full_stream`, `strong_curve_n1`, `end_to_end`"),
     (r"r06_bench_cfg2_steps20\.json", "the same command as the driver runs it (`--steps 20 --warmup 3`)"),
     (r"r06_bench_(cfg3|cfg4|cfg5|hq48|hq44|dn8|cfg2_s16)\.json", "`bench.py` lines of the other workloads, same box and build"),
