@@ -365,7 +365,6 @@ static unsigned long long g_launch_count[CR_KERNEL_IDS];
    kHz + 14-19 %, 48 -> 44.1 kHz + 3-17 %; at 44.1 -> 8 kHz, where 32-byte frames halve the tile, - 11 to + 13 % (profiles/r04_padded_tiles_ab.log) */
 #define CR_PADDED_MAX_INCREMENT (2u << 16)
 #define CR_UP2_SLACK 144u
-#define CR_UP2_ENTRIES_BYTES 1280u
 /* k_up2 as an instance's default kernel: see plan_geometry */
 #define CR_UP_DEFAULT_MAX_INCREMENT (65536u / 8u)
 #define CR_UP_DEFAULT_MIN_INCREMENT (65536u / 13u)
@@ -1453,8 +1452,6 @@ static void plan_geometry(ClownResamplerAMD_Plan *plan)
 		{
 			uint32_t stage_bytes = ((uint32_t)wave_tile * unit + 15u) & ~15u;
 
-			if (stage_bytes < CR_UP2_ENTRIES_BYTES)
-				stage_bytes = CR_UP2_ENTRIES_BYTES;   /* (k_up2 parks a wave-tile's converted window there first: UP2_ENTRIES_BYTES, cr_kup.hpp) */
 			plan->lds_bytes = rows_bytes + (plan->threads / 64u) * (2u * 1024u + stage_bytes + 2u * CR_UP2_SLACK) + 16u;
 			plan->tile_frames = (uint32_t)wave_tile * 4u;
 			per_cu = (160u * 1024u) / plan->lds_bytes;
@@ -1881,7 +1878,7 @@ static void plan_brief_shape(const cr_device_ctx *ctx, ClownResamplerAMD_Plan *p
 
 /* k_int beside the plan's ordinary kernel: see the plan's `intk`. */
 /* k_seg for this plan?  The shape k_up2 is the kernel of (the instance's slot signs hold for every row), at the ratios where a tile's
-   window fits its registers and LDS entries; the float image of the rows is made once per store.  0 on success (available or not). */
+   window fits its registers and LDS entries; the image of the rows it reads is made once per store.  0 on success (available or not). */
 static int plan_seg_shape(const cr_device_ctx *ctx, ClownResamplerAMD_Plan *plan)
 {
 	uint32_t negmask = 0, pos_bits = 0, neg_bits = 0, threads = 0, lds = 0, chunk = 0;
@@ -1914,11 +1911,7 @@ static int plan_seg_shape(const cr_device_ctx *ctx, ClownResamplerAMD_Plan *plan
 			const int32_t *row = plan->poly.weights + (size_t)r * plan->poly.row_stride;
 
 			for (s = 0; s < 15u; ++s)
-			{
-				/* |weight| <= 65536: exact as a float, and so is the division by 2^16 */
-				const float f = (float)(row[s] < 0 ? -(int64_t)row[s] : (int64_t)row[s]) * (1.0f / 65536.0f);
-				memcpy(&image[r * 16u + s], &f, sizeof(f));
-			}
+				image[r * 16u + s] = (uint32_t)row[s];   /* (|weight| <= 65536: cr_poly_slots_reaching above) */
 			image[r * 16u + 15u] = 2u * (uint32_t)row[plan->poly.slots];   /* the reciprocal, doubled: k_up2's normalisation (cr_kup.hpp) */
 		}
 		/* k_seg is an OPTIONAL fast path: whatever fails here leaves the plan without it (k_up2 / k_wave2 serve the configuration), and the

@@ -45,7 +45,7 @@ typedef struct cr_plan_store
 	int32_t *d_table;       /* caller's table as int32 (generic kernel) */
 	cr_poly poly;           /* host copy of the rows + row-index form (owns its arrays) */
 	int32_t *d_rows;        /* device image of the rows, NULL until a plan needs it */
-	void *d_rows_seg;       /* k_seg's image of the same rows (64 bytes per row: 15 x |weight| / 65536 as float, 2 * reciprocal), NULL until a plan needs it */
+	void *d_rows_seg;       /* k_seg's image of the same rows (64 bytes per row: 15 weights, 2 * reciprocal), NULL until a plan needs it */
 	int rows_layout;        /* CR_IMAGE_* of d_rows */
 	uint32_t plane_rows, swizzle, device_row_stride;
 } cr_plan_store;

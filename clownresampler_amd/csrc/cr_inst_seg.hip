@@ -10,8 +10,8 @@ namespace
 constexpr int SEG_WAVES = 12;
 typedef void (*seg_fn)(const crhip_seg_launch);
 // One shape of the one instance (stereo, 15 slots, pure upsampling): lines of 16 frames per lane and a ring of four groups - the ratios from 4x
-// up, which advance at most once in four frames (4.5x ... 16x: 85-103 us per 40 M output frames where k_wave2 / k_up2 take 93-128,
-// profiles/r05_seg_ratio_sweep.log).  The kernel is parameterised for more: with half-line chunks of 8 frames and a ring of eight groups it
+// up, which advance at most once in four frames (4.5x ... 16x: 93-104 us per 40 M output frames where k_wave2 / k_up2 take 104-128,
+// profiles/integer_chain_ratio_sweeps.log).  The kernel is parameterised for more: with half-line chunks of 8 frames and a ring of eight groups it
 // takes every ratio below 1:1 (bit-exact: tests ran it at 44.1 -> 48 kHz, 1.45x, 2.76x), but its half-line stores make it 149 us where
 // k_wave2 takes 95 on the 8-lobe 44.1 -> 48 kHz workload, non-temporal or not (profiles/r05_kseg_hq48_first.log): not instantiated.
 struct seg_shape

@@ -17,8 +17,8 @@ namespace
 // the same row, windows exactly D = S * increment / 65536 input frames apart.  Here the 64 lanes of a wave take the frames
 // j, j + S, ..., j + 63 S - lane l walks segment l of a "super-block" of 64 S output frames - so at every step the whole wave needs
 // ONE row, and:
-//   * the row arrives by s_load_dwordx16 (from a 64-byte-per-row float image in global memory: L2 / scalar cache), a frame ahead,
-//     and the taps take their weights as SCALAR operands of v_pk_fma_f32 (k_up2's FP32 round-toward-zero chain, cr_kup.hpp):
+//   * the row arrives by s_load_dwordx16 (from a 64-byte-per-row image in global memory: L2 / scalar cache), a frame ahead,
+//     and the taps take their weights as SCALAR operands of the 64-bit multiply-add:
 //     no row in LDS (66 KB free), no row address arithmetic in the vector unit, the fraction walk (g -= increment, wrap) is SALU;
 //   * every lane is at the same place in its window: "the position advances" is a scalar branch, the window a register ring -
 //     the frame body exists in TT rotations of the register names, so nothing is ever moved - fed one input frame per advance;
@@ -46,8 +46,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 {
 	static_assert(TT == 15 && NEGMASK == 0x2A55u, "the frame body is written out for 15 slots, slots 0, 2, 4, 6, 9, 11, 13 negative");
 	static_assert((CHUNK == 16u || CHUNK == 8u) && (NG & (NG - 1u)) == 0 && NG >= 4u, "a line or half a line per lane and chunk; a power of two of ring groups, the first window's four at least");
-	typedef float f32x2 __attribute__((ext_vector_type(2)));
-	typedef float f32x16 __attribute__((ext_vector_type(16)));
+	typedef int i32x16 __attribute__((ext_vector_type(16)));
 	constexpr unsigned LANE_STRIDE = seg_lane_stride(CHUNK);
 	constexpr unsigned WAVE_BYTES = seg_wave_bytes(CHUNK, NG);
 	constexpr unsigned PER_STORE = 64u / CHUNK;   // segments one store instruction covers (CHUNK lanes, 8 bytes each, per segment)
@@ -136,7 +135,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 	// input frames a chunk can advance over, at most: what the ring must hold ahead of the wave (see top_up)
 	const unsigned chunk_advances = (65535u + CHUNK * increment) >> 16;
 	// (constant address space: a uniform load from it is an s_load whatever the kernel stores elsewhere)
-	const __attribute__((address_space(4))) f32x16 *rows = (const __attribute__((address_space(4))) f32x16 *)(uintptr_t)a.d_rows;
+	const __attribute__((address_space(4))) i32x16 *rows = (const __attribute__((address_space(4))) i32x16 *)(uintptr_t)a.d_rows;
 	const uint64_t in_base = reinterpret_cast<uint64_t>(a.d_in);
 	const __amdgpu_buffer_rsrc_t in_rsrc = __builtin_amdgcn_make_buffer_rsrc(
 	    reinterpret_cast<void *>(((uint64_t)__builtin_amdgcn_readfirstlane((int)(unsigned)(in_base >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)in_base)), 0,
@@ -144,30 +143,24 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 	// lane l's window lies l * D input frames behind lane 0's (4 bytes per stereo frame; the host keeps everything below 2^32)
 	const unsigned lane_in_bytes = lane * (unsigned)a.seg_in_frames * 4u;
 
-	// {max(v, 0), max(-v, 0)} of both channels of a packed input frame, as floats: the sample's positive and negative part, both as magnitudes
-	auto convert = [&](int packed, f32x2 &left, f32x2 &right) {
-		float v0, v1;
-		asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_0" : "=v"(v0) : "v"(packed));
-		asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_1" : "=v"(v1) : "v"(packed));
-		asm("v_max_f32_e64 %0, %1, 0" : "=v"(left.x) : "v"(v0));
-		asm("v_max_f32_e64 %0, -%1, 0" : "=v"(left.y) : "v"(v0));
-		asm("v_max_f32_e64 %0, %1, 0" : "=v"(right.x) : "v"(v1));
-		asm("v_max_f32_e64 %0, -%1, 0" : "=v"(right.y) : "v"(v1));
+	// Both channels of a packed input frame as the taps take them: S = sample << 16 and its sign B = S >> 31.  The tap is k_up2's 64-bit
+	// multiply-add (cr_kup.hpp), P = S * weight + P on a pair {lo, hi} whose low half is armed for every tap: the product is a multiple of
+	// 65536, its integer part lands in `hi`, and a `lo` of all ones carries into `hi` exactly when the fraction is not zero - which is what
+	// a NEGATIVE product needs to be truncated as C truncates it (clownresampler.h:1020 via :625); a `lo` of 0 never does.  The window's
+	// registers rotate through the slots, so the weights keep their sign and the arm makes up for it: B for a slot whose weights are
+	// >= 0, ~B for one whose weights are <= 0 (a move or a not: one instruction either way; a sample of 0 has no fraction to carry).
+	auto convert = [&](int packed, int (&S)[2], int (&B)[2]) {
+		asm("v_lshlrev_b32 %0, 16, %1" : "=v"(S[0]) : "v"(packed));
+		asm("v_and_b32 %0, 0xffff0000, %1" : "=v"(S[1]) : "v"(packed));
+		asm("v_ashrrev_i32 %0, 31, %1" : "=v"(B[0]) : "v"(S[0]));
+		asm("v_ashrrev_i32 %0, 31, %1" : "=v"(B[1]) : "v"(S[1]));
 	};
 
-	// Where a frame's two chains start: 2^23, ulp 1 (cr_kup.hpp, FCHAIN).  Unlike k_up2, BOTH chains count upwards: one sums the products that
-	// are positive, the other the MAGNITUDES of the negative ones (a sample's negative part is kept as a magnitude, a slot with negative weights
-	// - staged as magnitudes too - takes the pair swapped: negative part x |weight| to the first chain, positive part x |weight| to the second).
-	// Round-toward-zero truncates either sum as C truncates the products (clownresampler.h:1020 via :625), and the frame's sum is the difference
-	// of the two accumulators' BITS (same exponent): one subtraction per channel, no sign to patch.
-	f32x2 chain_base;
-	chain_base.x = 8388608.0f;
-	chain_base.y = 8388608.0f;
-	asm volatile("" : "+v"(chain_base));
 	int thirty_one = 31;
 	asm volatile("" : "+v"(thirty_one));
-	int zero_c = 0, zero_d = 0;
-	asm volatile("" : "+{v117}"(zero_c), "+{v119}"(zero_d));   // the high halves of the normalisation's pinned addend pairs (see k_up2)
+	// the high halves of the pinned addend pairs: those of a frame's first taps, and the normalisation's (see k_up2)
+	int zero_a = 0, zero_b = 0, zero_c = 0, zero_d = 0;
+	asm volatile("" : "+{v113}"(zero_a), "+{v115}"(zero_b), "+{v117}"(zero_c), "+{v119}"(zero_d));
 
 	// staging: this lane's row, and where it reads for the copy-out (store i of a chunk: segments 4 i ... 4 i + 3, 16 lanes each)
 	// a lane's staging row: 8 bytes that take the write of "no frame yet", then its CHUNK frames
@@ -239,10 +232,10 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 		// (the previous tile's last stores are older than these requests: all of it has to land - once per tile)
 		asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 		const unsigned drawn = draw_ticket_end(ticket);
-		f32x2 P[TT][2];   // slot s of rotation R is P[(s + R) % TT]
+		int S_[TT][2], B_[TT][2];   // slot s of rotation R is [(s + R) % TT]
 #pragma unroll
 		for (int s = 0; s < TT; ++s)
-			convert(raw[s], P[s][0], P[s][1]);
+			convert(raw[s], S_[s], B_[s]);
 		mark(0);
 		if constexpr (ABL == 6)
 			phase[7] += 1;
@@ -266,11 +259,11 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 		int next_frame = 0;         // the frame the next advance brings in (read from LDS a position ahead)
 
 		// The row of a frame: (65536 - fraction) >> 6 (pure-upsampling row index), 64 bytes per row: s_load_dwordx16, a frame ahead.
-		auto load_row = [&](unsigned fraction_hi) -> f32x16 {
+		auto load_row = [&](unsigned fraction_hi) -> i32x16 {
 			const unsigned off = (0x10000u - (fraction_hi >> 16)) & 0x1FFC0u;
-			return *reinterpret_cast<const __attribute__((address_space(4))) f32x16 *>(reinterpret_cast<const __attribute__((address_space(4))) unsigned char *>(rows) + off);
+			return *reinterpret_cast<const __attribute__((address_space(4))) i32x16 *>(reinterpret_cast<const __attribute__((address_space(4))) unsigned char *>(rows) + off);
 		};
-		f32x16 w_a = load_row(F);
+		i32x16 w_a = load_row(F);
 
 		// bytes from the tile's first frame (segment 0) to the end of the stream, as far as 32 bits see (the host keeps a whole
 		// super-block - 64 S frames of 8 bytes - below 2^32, so whatever is clamped away here lies beyond every store of the tile)
@@ -328,54 +321,59 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 		};
 
 		// one frame of every lane with the window in rotation R; the weights: the scalar row `w`
-		auto frame = [&](auto r_tag, const f32x16 &w) {
+		auto frame = [&](auto r_tag, const i32x16 &w) {
 			constexpr int R = decltype(r_tag)::value;
-			auto wpair = [&](int k) {
-				f32x2 wp;
-				wp.x = w[2 * k];
-				wp.y = w[2 * k + 1];
-				return wp;
-			};
-#define CR_SEL_EP " op_sel_hi:[1,0,1]\n\t"
-#define CR_SEL_OP " op_sel:[0,1,0] op_sel_hi:[1,1,1]\n\t"
-#define CR_SEL_EN " op_sel:[1,0,0] op_sel_hi:[0,0,1]\n\t"
-#define CR_SEL_ON " op_sel:[1,1,0] op_sel_hi:[0,1,1]\n\t"
-#define CR_T(acc, p, wq, SEL) "v_pk_fma_f32 %" #acc ", %" #p ", %" #wq ", %" #acc SEL
-#define CR_F(acc, p, wq, base, SEL) "v_pk_fma_f32 %" #acc ", %" #p ", %" #wq ", %" #base SEL
-#define CR_P(s, c) P[((s) + R) % TT][c]
-			f32x2 a0, a1;
-			// slots 0 (-), 1 (+), 2 (-), 3 (+), 4 (-), 5 (+), 6 (-), 7 (+): cr_kup.hpp, the same strings with scalar weight pairs
-			asm volatile(CR_F(0, 2, 18, 22, CR_SEL_EN) CR_F(1, 10, 18, 22, CR_SEL_EN) CR_T(0, 3, 18, CR_SEL_OP) CR_T(1, 11, 18, CR_SEL_OP)
-			             CR_T(0, 4, 19, CR_SEL_EN) CR_T(1, 12, 19, CR_SEL_EN) CR_T(0, 5, 19, CR_SEL_OP) CR_T(1, 13, 19, CR_SEL_OP)
-			             CR_T(0, 6, 20, CR_SEL_EN) CR_T(1, 14, 20, CR_SEL_EN) CR_T(0, 7, 20, CR_SEL_OP) CR_T(1, 15, 20, CR_SEL_OP)
-			             CR_T(0, 8, 21, CR_SEL_EN) CR_T(1, 16, 21, CR_SEL_EN) CR_T(0, 9, 21, CR_SEL_OP) CR_T(1, 17, 21, CR_SEL_OP)
-			             : "=&v"(a0), "=&v"(a1)
-			             : "v"(CR_P(0, 0)), "v"(CR_P(1, 0)), "v"(CR_P(2, 0)), "v"(CR_P(3, 0)), "v"(CR_P(4, 0)), "v"(CR_P(5, 0)), "v"(CR_P(6, 0)), "v"(CR_P(7, 0)),
-			               "v"(CR_P(0, 1)), "v"(CR_P(1, 1)), "v"(CR_P(2, 1)), "v"(CR_P(3, 1)), "v"(CR_P(4, 1)), "v"(CR_P(5, 1)), "v"(CR_P(6, 1)), "v"(CR_P(7, 1)),
-			               "s"(wpair(0)), "s"(wpair(1)), "s"(wpair(2)), "s"(wpair(3)), "v"(chain_base));
+			// Four slots per statement (an asm statement takes at most 30 operands; between statements hipcc pads, inside one the hardware
+			// interlocks).  The accumulator pairs are v[120:121] and v[124:125]; the first slot's taps add to {arm, 0} in v[112:113] and
+			// v[114:115].  M / N: the slot's weights are >= 0 / <= 0.
+#define CR_S(s, c) "v"(S_[((s) + R) % TT][c])
+#define CR_B(s, c) "v"(B_[((s) + R) % TT][c])
+#define CR_W(s) "s"(w[s])
+#define CR_M "v_mov_b32"
+#define CR_N "v_not_b32"
+#define CR_TAP(ARM, s0, s1, b0, b1, wt)                                                                                            \
+	ARM " v120, %" #b0 "\n\t" ARM " v124, %" #b1 "\n\t"                                                                            \
+	"v_mad_i64_i32 v[120:121], vcc, %" #s0 ", %" #wt ", v[120:121]\n\t"                                                            \
+	"v_mad_i64_i32 v[124:125], vcc, %" #s1 ", %" #wt ", v[124:125]\n\t"
+#define CR_FOUR(s) CR_S(s, 0), CR_S(s, 1), CR_S(s + 1, 0), CR_S(s + 1, 1), CR_S(s + 2, 0), CR_S(s + 2, 1), CR_S(s + 3, 0), CR_S(s + 3, 1),      \
+	CR_B(s, 0), CR_B(s, 1), CR_B(s + 1, 0), CR_B(s + 1, 1), CR_B(s + 2, 0), CR_B(s + 2, 1), CR_B(s + 3, 0), CR_B(s + 3, 1),                \
+	CR_W(s), CR_W(s + 1), CR_W(s + 2), CR_W(s + 3)
+			int hi0, hi1;
+			// slots 0 (-), 1 (+), 2 (-), 3 (+)
+			asm volatile(CR_N " v112, %10\n\t" CR_N " v114, %11\n\t"
+			             "v_mad_i64_i32 v[120:121], vcc, %2, %18, v[112:113]\n\t"
+			             "v_mad_i64_i32 v[124:125], vcc, %3, %18, v[114:115]\n\t"
+			             CR_TAP(CR_M, 4, 5, 12, 13, 19) CR_TAP(CR_N, 6, 7, 14, 15, 20) CR_TAP(CR_M, 8, 9, 16, 17, 21)
+			             : "=&{v121}"(hi0), "=&{v125}"(hi1)
+			             : CR_FOUR(0), "{v113}"(zero_a), "{v115}"(zero_b)
+			             : "vcc", "v112", "v114", "v120", "v124");
+			// slots 4 (-), 5 (+), 6 (-), 7 (+)
+			asm volatile(CR_TAP(CR_N, 2, 3, 10, 11, 18) CR_TAP(CR_M, 4, 5, 12, 13, 19) CR_TAP(CR_N, 6, 7, 14, 15, 20) CR_TAP(CR_M, 8, 9, 16, 17, 21)
+			             : "+{v121}"(hi0), "+{v125}"(hi1)
+			             : CR_FOUR(4)
+			             : "vcc", "v120", "v124");
 			write_pending();   // the previous frame's result: its LDS write has the rest of this frame to complete
-			// slots 8 (+), 9 (-), 10 (+), 11 (-), 12 (+), 13 (-), 14 (+)
-			asm volatile(CR_T(0, 2, 16, CR_SEL_EP) CR_T(1, 9, 16, CR_SEL_EP) CR_T(0, 3, 16, CR_SEL_ON) CR_T(1, 10, 16, CR_SEL_ON)
-			             CR_T(0, 4, 17, CR_SEL_EP) CR_T(1, 11, 17, CR_SEL_EP) CR_T(0, 5, 17, CR_SEL_ON) CR_T(1, 12, 17, CR_SEL_ON)
-			             CR_T(0, 6, 18, CR_SEL_EP) CR_T(1, 13, 18, CR_SEL_EP) CR_T(0, 7, 18, CR_SEL_ON) CR_T(1, 14, 18, CR_SEL_ON)
-			             CR_T(0, 8, 19, CR_SEL_EP) CR_T(1, 15, 19, CR_SEL_EP)
-			             : "+v"(a0), "+v"(a1)
-			             : "v"(CR_P(8, 0)), "v"(CR_P(9, 0)), "v"(CR_P(10, 0)), "v"(CR_P(11, 0)), "v"(CR_P(12, 0)), "v"(CR_P(13, 0)), "v"(CR_P(14, 0)),
-			               "v"(CR_P(8, 1)), "v"(CR_P(9, 1)), "v"(CR_P(10, 1)), "v"(CR_P(11, 1)), "v"(CR_P(12, 1)), "v"(CR_P(13, 1)), "v"(CR_P(14, 1)),
-			               "s"(wpair(4)), "s"(wpair(5)), "s"(wpair(6)), "s"(wpair(7)));
-#undef CR_P
-#undef CR_F
-#undef CR_T
-#undef CR_SEL_ON
-#undef CR_SEL_EN
-#undef CR_SEL_OP
-#undef CR_SEL_EP
-			// first chain = 2^23 + p, second = 2^23 + q: the frame's sum is p - q
-			const int hi0 = (int)(__float_as_uint(a0.x) - __float_as_uint(a0.y));
-			const int hi1 = (int)(__float_as_uint(a1.x) - __float_as_uint(a1.y));
+			// slots 8 (+), 9 (-), 10 (+), 11 (-)
+			asm volatile(CR_TAP(CR_M, 2, 3, 10, 11, 18) CR_TAP(CR_N, 4, 5, 12, 13, 19) CR_TAP(CR_M, 6, 7, 14, 15, 20) CR_TAP(CR_N, 8, 9, 16, 17, 21)
+			             : "+{v121}"(hi0), "+{v125}"(hi1)
+			             : CR_FOUR(8)
+			             : "vcc", "v120", "v124");
+			// slots 12 (+), 13 (-), 14 (+)
+			asm volatile(CR_TAP(CR_M, 2, 3, 8, 9, 14) CR_TAP(CR_N, 4, 5, 10, 11, 15) CR_TAP(CR_M, 6, 7, 12, 13, 16)
+			             : "+{v121}"(hi0), "+{v125}"(hi1)
+			             : CR_S(12, 0), CR_S(12, 1), CR_S(13, 0), CR_S(13, 1), CR_S(14, 0), CR_S(14, 1), CR_B(12, 0), CR_B(12, 1), CR_B(13, 0), CR_B(13, 1), CR_B(14, 0), CR_B(14, 1),
+			               CR_W(12), CR_W(13), CR_W(14)
+			             : "vcc", "v120", "v124");
+#undef CR_FOUR
+#undef CR_TAP
+#undef CR_N
+#undef CR_M
+#undef CR_W
+#undef CR_B
+#undef CR_S
 			// (acc * reciprocal) / 32768 toward zero (clownresampler.h:1033), the row's last entry being 2 * reciprocal: k_up2's form
 			int out0, out1;
-			const int reciprocal2 = (int)__float_as_uint(w[TT]);
+			const int reciprocal2 = w[TT];
 			asm("v_ashrrev_i32_sdwa v116, %4, %2 dst_sel:WORD_0 dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:DWORD\n\t"
 			    "v_ashrrev_i32_sdwa v118, %4, %3 dst_sel:WORD_0 dst_unused:UNUSED_PAD src0_sel:DWORD src1_sel:DWORD\n\t"
 			    "v_mad_i64_i32 v[122:123], vcc, %2, %5, v[116:117]\n\t"
@@ -388,11 +386,6 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 			pending.x = out0;
 			pending.y = out1;
 		};
-
-		// FP32 rounding: toward zero, for the chains - and the mode the wave came with put back behind the tile (not a
-		// hard-coded 0).  Nothing between the two but the kernel's own asm arithmetic and integer / scalar code.
-		unsigned fp_mode;
-		asm volatile("s_getreg_b32 %0, hwreg(HW_REG_MODE, 0, 2)\n\ts_setreg_imm32_b32 hwreg(HW_REG_MODE, 0, 2), 3" : "=s"(fp_mode));
 
 		// the frame the first advance brings in
 		// entry TT + k is the frame advance k + 1 brings in: [group mod NG][lane][entry mod 4]
@@ -420,7 +413,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 							asm volatile("" : "+s"(w_a));
 							mark(1);
 						}
-						f32x16 w_next = w_a;
+						i32x16 w_next = w_a;
 						if constexpr (ABL != 1 && ABL != 3)
 							w_next = load_row(next);
 						frame(r_tag, w_a);
@@ -460,7 +453,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 					{
 						mark(-1);
 						// the position advances: the oldest slot's registers take the new frame, the names rotate by one
-						convert(next_frame, P[R % TT][0], P[R % TT][1]);
+						convert(next_frame, S_[R % TT], B_[R % TT]);
 						++advance;
 						next_frame = *reinterpret_cast<const __attribute__((address_space(3))) int *>((uintptr_t)entry_at((unsigned)TT + advance));
 						mark(5);
@@ -468,8 +461,6 @@ __global__ __launch_bounds__(WAVES * 64) void k_seg(const crhip_seg_launch a)
 				}
 			});
 		}
-
-		asm volatile("s_setreg_b32 hwreg(HW_REG_MODE, 0, 2), %0" ::"s"(fp_mode));
 
 		const uint64_t next = draw_resolve(drawn);
 		if (next == ~0ull)

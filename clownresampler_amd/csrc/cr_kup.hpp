@@ -444,23 +444,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_up(const crhip_poly_launch a)
 // ---------------------------------------------------------------------------------------------------------
 // bytes of slack on either side of a wave's staging buffer (16 surplus frames of 8 bytes, rounded up to 16 bytes)
 constexpr unsigned UP2_SLACK = 144u;
-// the least a wave's staging buffer holds: 80 converted input frames of 16 bytes (64 positions + a window of up to 16 slots)
-constexpr unsigned UP2_ENTRIES_BYTES = 1280u;
-//
-// FCHAIN = 1: the tap as ONE instruction, on the FLOAT pipe (round 4).  An FP32 accumulator that starts at 2^23 has an ulp of exactly 1,
-// and under round-toward-zero fma(|v|, |w| / 65536, acc) = acc + floor(|v| |w| / 65536): the product is exact inside the fused
-// operation (15 x 17 bits), the sum is rounded once, toward zero = downward for a positive sum - C's truncating division
-// (clownresampler.h:1020 via :625) of a non-negative product, accumulated, no arming, no 64-bit pair.  A negative product
-// truncates toward zero the same way on an accumulator that starts at -2^23.  Which of the two a tap feeds is the sign of
-// sample x weight - the weight's sign is the slot's (NEGMASK), the sample's is known once per window - so the window is
-// unpacked into pairs {max(v, 0), min(v, 0)} of v = +-sample as floats, the rows are staged as |weight| / 65536 (exact: at most
-// 17 bits), and v_pk_fma_f32 advances BOTH chains of a channel in one instruction (one of the two adds zero).  The frame's sum is
-// (bits of the positive chain) - (bits of the negative chain) + 2^31.  No slot is special (a weight of 65536 is 1.0f), nothing is
-// pinned.  |sum| < 2^23 is what the host proves for every 32-bit kernel; the chains' partial sums are bounded by the sum of
-// |weight| x 2^15 / 65536 < 2^19 for any table the 32-bit kernels accept.  tools/microbench/rtzchain.hip checks 2.7e8 random
-// 15-tap frames against the integer definition (0 differ) and tools/microbench/valurate.hip prices the instructions:
-// v_pk_fma_f32 2.0 ns per wave-instruction and SIMD at this occupancy against 2.95 for v_mov_b32 + v_mad_i64_i32.
-template <int CH, int TT, int NORM, unsigned NEGMASK, int WAVES, int OUT16, int NT, int ABL = 0, int FCHAIN = 0>
+template <int CH, int TT, int NORM, unsigned NEGMASK, int WAVES, int OUT16, int NT, int ABL = 0>
 __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 {
 	static_assert(CH == 2, "k_up2 is written for stereo (one packed dword per input frame, two accumulator pairs)");
@@ -517,10 +501,8 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 	};
 
 	const unsigned WT = a.tile_frames / 4u;        // output frames per wave-tile: at most 64 input positions
-	// (at least UP2_ENTRIES_BYTES: the float chain parks the wave-tile's converted input frames there before the first frame is staged)
-	const unsigned stage_bytes = ((WT * UNIT + 15u) & ~15u) > UP2_ENTRIES_BYTES ? ((WT * UNIT + 15u) & ~15u) : UP2_ENTRIES_BYTES;
+	const unsigned stage_bytes = (WT * UNIT + 15u) & ~15u;
 	static_assert(17u * UNIT <= UP2_SLACK, "slack for a lane's surplus frames on either side of the staged tile");
-	static_assert((64u + TT - 1u) * 16u <= UP2_ENTRIES_BYTES, "one 16-byte entry per input frame of a wave-tile's window");
 
 	// per wave: two window buffers, slack, the staged frames of a wave-tile, slack (the host sizes the workgroup's LDS for this:
 	// cr_context.c, plan_geometry)
@@ -563,9 +545,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 					for (int j = 0; j < 4; ++j)
 					{
 						const int slot = 4 * q + j;
-						if (slot < TT && FCHAIN)
-							e[j] = (int)__float_as_uint((float)(e[j] < 0 ? -e[j] : e[j]) * (1.0f / 65536.0f));   // |weight| / 65536 as a float: exact
-						else if (slot < TT)
+						if (slot < TT)
 							e[j] = mad_staged_weight<TT, NEGMASK>(e[j], slot);   // |weight| << 15; the centre slots: the weight as it is
 						else if (slot == TT && NORM == CRHIP_NORM_U32)
 							e[j] = 2 * e[j];   // the reciprocal, doubled: see the normalisation in `one`
@@ -688,63 +668,14 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 
 		// the window of this lane's input position, once: X = +-2 * sample (operand AND arm of the ordinary slots); the centre
 		// slots: S = sample << 16 and its sign B
-		typedef float f32x2 __attribute__((ext_vector_type(2)));
-		typedef float f32x4 __attribute__((ext_vector_type(4)));
-		f32x2 P[FCHAIN ? TT : 1][CH];   // FCHAIN: {max(v, 0), min(v, 0)} of v = the sample of window frame s, channel c
-		int f[FCHAIN ? 1 : TT];
-		if constexpr (FCHAIN)
-		{
-			// The windows of neighbouring lanes overlap in all but one frame, so every input frame of the wave-tile is converted ONCE -
-			// lane l converts frames l and 64 + l (the window of the last lane ends at frame 63 + TT - 1) - into {max(v, 0), min(v, 0)}
-			// per channel, 16 bytes, parked in the staging buffer (free until the first frame is staged: the LDS operations of a wave
-			// complete in order), and every lane then reads its TT entries back: 12 VALU per wave-tile where a lane converting its own
-			// window took 90.  A slot whose weights are negative takes the pair swapped and negated, which the multiply-add does for
-			// free (op_sel / neg_lo / neg_hi): {max(-v, 0), min(-v, 0)} = {-min(v, 0), -max(v, 0)}.
-			static_assert(64 + 63 < (int)(BUF / FB) && TT <= 64 && (2u * BUF + UP2_SLACK) % 16u == 0, "the second frame of every lane lies inside the window buffer; 16-byte entries");
-			auto convert = [&](int packed) {
-				float v0, v1;
-				f32x4 e;
-				asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_0" : "=v"(v0) : "v"(packed));
-				asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:WORD_1" : "=v"(v1) : "v"(packed));
-				asm("v_max_f32_e64 %0, %1, 0" : "=v"(e.x) : "v"(v0));
-				asm("v_min_f32_e64 %0, %1, 0" : "=v"(e.y) : "v"(v0));
-				asm("v_max_f32_e64 %0, %1, 0" : "=v"(e.z) : "v"(v1));
-				asm("v_min_f32_e64 %0, %1, 0" : "=v"(e.w) : "v"(v1));
-				return e;
-			};
-			f32x4 *entries = reinterpret_cast<f32x4 *>(my_stage);
-			const int own = *reinterpret_cast<const int *>(base + lane * FB);
-			const int beyond = *reinterpret_cast<const int *>(base + (64u + lane) * FB);   // (lanes from TT - 1 on: past the window, never read back)
-			entries[lane] = convert(own);
-			if (lane < (unsigned)TT - 1u)
-				entries[64u + lane] = convert(beyond);
-			__builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-			__builtin_amdgcn_wave_barrier();
-			__builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+		int f[TT];
 #pragma unroll
-			for (int s = 0; s < TT; ++s)
-			{
-				const f32x4 e = entries[lane + (unsigned)s];
-				P[s][0].x = e.x;
-				P[s][0].y = e.y;
-				P[s][1].x = e.z;
-				P[s][1].y = e.w;
-			}
-			// (the frames' staging writes below come after these reads: same wave, in order)
-			__builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-			__builtin_amdgcn_wave_barrier();
-			__builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-		}
-		else
-		{
-#pragma unroll
-			for (int s = 0; s < TT; ++s)
-				f[s] = *reinterpret_cast<const int *>(base + (lane + (unsigned)s) * FB);
-		}
+		for (int s = 0; s < TT; ++s)
+			f[s] = *reinterpret_cast<const int *>(base + (lane + (unsigned)s) * FB);
 		int X[TT][CH], B[TT][CH];
 		int plus_two = 2, minus_two = -2;
 #pragma unroll
-		for (int s = 0; s < (FCHAIN ? 0 : TT); ++s)
+		for (int s = 0; s < TT; ++s)
 		{
 			if ((SAFEMASK >> s) & 1u)
 			{
@@ -802,10 +733,6 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 			}
 		};
 
-		f32x2 chain_base;   // FCHAIN: where a frame's two chains start
-		chain_base.x = 8388608.0f;
-		chain_base.y = -8388608.0f;
-		asm volatile("" : "+v"(chain_base));
 		// PRED: the frame is stored only by the lanes with `extra`
 		auto one = [&](const int (&w)[RS], auto pred_tag) {
 			constexpr bool PRED = decltype(pred_tag)::value;
@@ -822,72 +749,6 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 			// different register (static_assert(TT > 1) above; tests/test_gpu_parity.py::test_input_stationary_* run every instance
 			// against the oracle).
 			int lo0, hi0, lo1, hi1;
-			if constexpr (FCHAIN)
-			{
-				// one v_pk_fma_f32 per tap and channel: {positive chain, negative chain} += {max(v, 0), min(v, 0)} * (|weight| / 65536),
-				// round toward zero (set around the frame loop); the weight is the low or the high half of a register pair of the row
-				// (Written as one or two asm statements, not one per tap: between asm statements that touch a common register hipcc pads
-				// with s_nop - 10 per frame here - while dependent VALU instructions inside a statement need none: the hardware
-				// interlocks them.  An asm statement takes at most 30 operands: 15 slots are two statements.)
-				f32x2 a0, a1;
-				auto wpair = [&](int k) {
-					f32x2 wp;
-					wp.x = __uint_as_float((unsigned)w[2 * k]);
-					wp.y = __uint_as_float((unsigned)w[2 * k + 1]);
-					return wp;
-				};
-// E / O: the weight is the low / high half of its register pair; P / N: the slot's weights are >= 0 / <= 0 (N: the sample pair swapped
-// and negated); F: the first tap of a frame, which adds to the chains' base
-#define CR_SEL_EP " op_sel_hi:[1,0,1]\n\t"
-#define CR_SEL_OP " op_sel:[0,1,0] op_sel_hi:[1,1,1]\n\t"
-#define CR_SEL_EN " op_sel:[1,0,0] op_sel_hi:[0,0,1] neg_lo:[1,0,0] neg_hi:[1,0,0]\n\t"
-#define CR_SEL_ON " op_sel:[1,1,0] op_sel_hi:[0,1,1] neg_lo:[1,0,0] neg_hi:[1,0,0]\n\t"
-#define CR_T(acc, p, wq, SEL) "v_pk_fma_f32 %" #acc ", %" #p ", %" #wq ", %" #acc SEL
-#define CR_F(acc, p, wq, base, SEL) "v_pk_fma_f32 %" #acc ", %" #p ", %" #wq ", %" #base SEL
-				if constexpr (TT == 15)
-				{
-					static_assert(NEGMASK == 0x2A55u, "slots 0, 2, 4, 6, 9, 11, 13 negative: the strings below are written for this mask");
-					asm volatile(CR_F(0, 2, 18, 22, CR_SEL_EN) CR_F(1, 10, 18, 22, CR_SEL_EN) CR_T(0, 3, 18, CR_SEL_OP) CR_T(1, 11, 18, CR_SEL_OP)
-					             CR_T(0, 4, 19, CR_SEL_EN) CR_T(1, 12, 19, CR_SEL_EN) CR_T(0, 5, 19, CR_SEL_OP) CR_T(1, 13, 19, CR_SEL_OP)
-					             CR_T(0, 6, 20, CR_SEL_EN) CR_T(1, 14, 20, CR_SEL_EN) CR_T(0, 7, 20, CR_SEL_OP) CR_T(1, 15, 20, CR_SEL_OP)
-					             CR_T(0, 8, 21, CR_SEL_EN) CR_T(1, 16, 21, CR_SEL_EN) CR_T(0, 9, 21, CR_SEL_OP) CR_T(1, 17, 21, CR_SEL_OP)
-					             : "=&v"(a0), "=&v"(a1)
-					             : "v"(P[0][0]), "v"(P[1][0]), "v"(P[2][0]), "v"(P[3][0]), "v"(P[4][0]), "v"(P[5][0]), "v"(P[6][0]), "v"(P[7][0]),
-					               "v"(P[0][1]), "v"(P[1][1]), "v"(P[2][1]), "v"(P[3][1]), "v"(P[4][1]), "v"(P[5][1]), "v"(P[6][1]), "v"(P[7][1]),
-					               "v"(wpair(0)), "v"(wpair(1)), "v"(wpair(2)), "v"(wpair(3)), "v"(chain_base));
-					// slots 8 (+), 9 (-), 10 (+), 11 (-), 12 (+), 13 (-), 14 (+)
-					asm volatile(CR_T(0, 2, 16, CR_SEL_EP) CR_T(1, 9, 16, CR_SEL_EP) CR_T(0, 3, 16, CR_SEL_ON) CR_T(1, 10, 16, CR_SEL_ON)
-					             CR_T(0, 4, 17, CR_SEL_EP) CR_T(1, 11, 17, CR_SEL_EP) CR_T(0, 5, 17, CR_SEL_ON) CR_T(1, 12, 17, CR_SEL_ON)
-					             CR_T(0, 6, 18, CR_SEL_EP) CR_T(1, 13, 18, CR_SEL_EP) CR_T(0, 7, 18, CR_SEL_ON) CR_T(1, 14, 18, CR_SEL_ON)
-					             CR_T(0, 8, 19, CR_SEL_EP) CR_T(1, 15, 19, CR_SEL_EP)
-					             : "+v"(a0), "+v"(a1)
-					             : "v"(P[8][0]), "v"(P[9][0]), "v"(P[10][0]), "v"(P[11][0]), "v"(P[12][0]), "v"(P[13][0]), "v"(P[14][0]),
-					               "v"(P[8][1]), "v"(P[9][1]), "v"(P[10][1]), "v"(P[11][1]), "v"(P[12][1]), "v"(P[13][1]), "v"(P[14][1]),
-					               "v"(wpair(4)), "v"(wpair(5)), "v"(wpair(6)), "v"(wpair(7)));
-				}
-				else
-				{
-					static_assert(TT == 5 && NEGMASK == 0x12u, "k_up2's float chain is written out for 15 slots (mask 0x2A55) and 5 slots (mask 0x12: slots 1 and 4 negative)");
-					asm volatile(CR_F(0, 2, 12, 15, CR_SEL_EP) CR_F(1, 7, 12, 15, CR_SEL_EP) CR_T(0, 3, 12, CR_SEL_ON) CR_T(1, 8, 12, CR_SEL_ON)
-					             CR_T(0, 4, 13, CR_SEL_EP) CR_T(1, 9, 13, CR_SEL_EP) CR_T(0, 5, 13, CR_SEL_OP) CR_T(1, 10, 13, CR_SEL_OP)
-					             CR_T(0, 6, 14, CR_SEL_EN) CR_T(1, 11, 14, CR_SEL_EN)
-					             : "=&v"(a0), "=&v"(a1)
-					             : "v"(P[0][0]), "v"(P[1][0]), "v"(P[2][0]), "v"(P[3][0]), "v"(P[4][0]),
-					               "v"(P[0][1]), "v"(P[1][1]), "v"(P[2][1]), "v"(P[3][1]), "v"(P[4][1]),
-					               "v"(wpair(0)), "v"(wpair(1)), "v"(wpair(2)), "v"(chain_base));
-				}
-#undef CR_F
-#undef CR_T
-#undef CR_SEL_ON
-#undef CR_SEL_EN
-#undef CR_SEL_OP
-#undef CR_SEL_EP
-				// positive chain = 2^23 + p (bits 0x4B000000 + p), negative chain = -(2^23 + q) (bits 0xCB000000 + q): p - q
-				hi0 = (int)(__float_as_uint(a0.x) - __float_as_uint(a0.y) + 0x80000000u);
-				hi1 = (int)(__float_as_uint(a1.x) - __float_as_uint(a1.y) + 0x80000000u);
-			}
-			else
-			{
 			asm("v_mad_i64_i32 v[120:121], vcc, %1, %2, v[112:113]" : "={v121}"(hi0) : "v"(X[0][0]), "v"(w[0]), "{v112}"(X[0][0]), "{v113}"(zero_a) : "vcc", "v120");
 			asm("v_mad_i64_i32 v[124:125], s[94:95], %1, %2, v[114:115]" : "={v125}"(hi1) : "v"(X[0][1]), "v"(w[0]), "{v114}"(X[0][1]), "{v115}"(zero_b) : "s94", "s95", "v124");
 #define CRHIP_UP2_TAP(LO, HI, VLO, VHI, SAMPLE, WEIGHT, ARM)                                                                        \
@@ -904,7 +765,6 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 			}
 #undef CRHIP_UP2_TAP_B
 #undef CRHIP_UP2_TAP
-			}
 			(void)lo0;
 			(void)lo1;
 
@@ -948,9 +808,6 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 		};
 
 		mark(0);
-		unsigned fp_mode = 0;   // (the wave's FP32 rounding mode is put back as it was found)
-		if constexpr (FCHAIN)
-			asm volatile("s_getreg_b32 %0, hwreg(HW_REG_MODE, 0, 2)\n\ts_setreg_imm32_b32 hwreg(HW_REG_MODE, 0, 2), 3" : "=s"(fp_mode));   // FP32 rounding: toward zero, for the chains of the frames
 		// the row of frame j + 1 is read before the arithmetic of frame j (two register sets, loop unrolled by two)
 		int wa[RS], wb[RS];
 		read_row(g, wa);
@@ -986,9 +843,6 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 		}
 		if (any_extra)
 			one(wa, std::true_type());   // (its row was read as the prefetch of the last trip)
-		if constexpr (FCHAIN)
-			asm volatile("s_setreg_b32 hwreg(HW_REG_MODE, 0, 2), %0" ::"s"(fp_mode));   // back to the mode the wave came with
-
 		mark(1);
 		// the staged frames of the other lanes: same wave, LDS operations of a wave complete in order
 		__builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");

@@ -144,8 +144,8 @@ typedef struct crhip_seg_launch
 	const void *d_in;           /* interleaved int16, stereo */
 	uint64_t in_valid_bytes;    /* < 2^32 */
 	void *d_out;                /* int32, n_out * 2 */
-	const void *d_rows;         /* the FLOAT row image: 16 dwords per row, row-major - |weight| / 65536 as float for the 15 slots, then
-	                               2 * reciprocal as int32 (clownresampler.h:1025, :1033) */
+	const void *d_rows;         /* the row image: 16 int32 per row, row-major - the weights of the 15 slots, then 2 * reciprocal
+	                               (clownresampler.h:1025, :1033) */
 	uint64_t pos0;              /* 16.16, of output frame 0 relative to frame 0 of d_in */
 	uint64_t n_out;
 	uint64_t seg_frames;        /* S: a multiple of 65536 / gcd(increment, 65536) and of tile_frames; 512 S < 2^32 */

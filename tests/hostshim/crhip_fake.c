@@ -645,7 +645,7 @@ int crhip_launch_int(const crhip_int_launch *l, void *stream)
 	return 0;
 }
 
-/* k_seg from its launch arguments: the float image of the rows (|weight| / 65536, then 2 x the reciprocal), the instance's slot signs, the
+/* k_seg from its launch arguments: the image of the rows (the weights, then 2 x the reciprocal), the instance's slot signs, the
    launch's tiling held to the rules the kernel's 32-bit arithmetic needs (cr_kseg.hpp; host: cr_context.c cr_plan_launch) */
 int crhip_launch_seg(const crhip_seg_launch *l, void *stream)
 {
@@ -695,13 +695,10 @@ int crhip_launch_seg(const crhip_seg_launch *l, void *stream)
 
 			for (s = 0; s < 15u; ++s)
 			{
-				float f;
-				int64_t weight;
+				const int64_t weight = (int32_t)image[row * 16u + s];
 
-				memcpy(&f, &image[row * 16u + s], sizeof(f));
-				weight = (int64_t)(f * 65536.0f);
-				if ((negmask >> s) & 1u)
-					weight = -weight;
+				if (((negmask >> s) & 1u) != 0 ? weight > 0 : weight < 0)   /* the kernel arms its taps by the slot's sign */
+					return FAKE_ERROR_LAUNCH;
 				acc += input_sample(l->d_in, l->in_valid_bytes, (first + s) * 2u + c) * weight / 65536;
 			}
 			((int32_t *)l->d_out)[j * 2u + c] = (int32_t)(acc * reciprocal / 32768);

@@ -480,13 +480,14 @@ def test_abort_on_error_is_opt_in(tmp_path):
 
 
 def test_device_code_keeps_its_promises(tmp_path):
-    """Reads the gfx950 code objects out of the built library and checks three things the kernels' comments rely on and hipcc is
+    """Reads the gfx950 code objects out of the built library and checks four things the kernels' comments rely on and hipcc is
     free to break behind the source's back:
     (1) no flat_ memory instruction anywhere: LDS words are addressed as LDS, global memory as global (a flat access counts in
         vmcnt AND lgkmcnt, and a volatile one is followed by vmcnt(0));
     (2) nothing is written through the scalar data cache: scalar memory instructions only load;
     (3) the VGPR of a ticket drawn with draw_ticket_begin (a returning vector atomic, result in flight) is not touched by ANY
-        instruction before an s_waitcnt on vmcnt, and in the tile loops that wait leaves the tile's own stores in flight."""
+        instruction before an s_waitcnt on vmcnt, and in the tile loops that wait leaves the tile's own stores in flight;
+    (4) no packed FP32 arithmetic: some forms of it have given wrong results on the target."""
     import shutil
     objdump = "/opt/rocm/lib/llvm/bin/llvm-objdump"
     if not os.path.exists(objdump):
@@ -505,6 +506,8 @@ def test_device_code_keeps_its_promises(tmp_path):
         assert not flat, (bundle.name, flat[:3])
         written = [l for l in lines if re.match(r"s_\w*(atomic|store|dcache_wb|dcache_discard)", l)]
         assert not written, (bundle.name, written[:3])
+        packed = [l for l in lines if re.match(r"v_pk_(add|mul|fma)_f32", l)]
+        assert not packed, (bundle.name, packed[:3])
         for i, line in enumerate(lines):
             m = re.match(r"global_atomic_add v(\d+), .*\bsc0\b", line)
             if not m:

@@ -27,6 +27,7 @@ for doc in ("DESIGN.md", "README.md", "INTEGRATION.md"):
 cited.pop("INDEX.md", None)   # (this file)
 missing = [n for n in cited if not os.path.exists(os.path.join(P, n))]
 WHAT = [
+    (r"integer_chain_ratio_sweeps\.log", "`k_seg` and `k_up2` on integer chains against the other kernels by upsampling ratio; cfg 3 and its shorter forms (`bench.py`)"),
     (r"vector_tickets_all_workloads\.log", "every workload of bench.py once, tickets drawn by vector atomics"),
     (r"vector_tickets_ab\.log", "ticketed against round-robin tiles in `k_poly`, same box, three times each in turn"),
     (r"r06_bench_cfg2\.json", "the headline `bench.py` line (BASELINE configs[1], N = 1) of round 6's final build, with `roofline`, `cpu_baseline`, `parity_full_stream`, `strong_curve_n1`, `end_to_end`"),
@@ -103,7 +104,7 @@ WHAT = [
     (r"r04_kup2_ab\.log", "cfg 3, same box: round 3's `k_up2`, round 4's with the integer chain, with the FP32 chain, with the shared window conversion"),
     (r"r04_kup2_frame\.s", "annotated disassembly of one `k_up2` frame"),
     (r"r04_kup2_ablations\.log", "`k_up2` timing-only ablations and in-kernel phase stamps"),
-    (r"r04_rtzchain\.log", "the FP32 round-toward-zero chain against the integer definition (2.7e8 frames), `tools/microbench/rtzchain.hip`"),
+    (r"r04_rtzchain\.log", "the FP32 round-toward-zero chain against the integer definition (2.7e8 frames), a microbenchmark since removed"),
     (r"r04_valurate\.log", "issue cost of the VALU instructions the taps are built from, `tools/microbench/valurate.hip`"),
     (r"r04_dual_mono_ab\.log", "dual mono against the mono kernels, same box"),
     (r"r04_three_group_tiles_ab\.log", "3,072-frame tiles against 2,048 (48 → 44.1 kHz shapes)"),

@@ -9,7 +9,7 @@ typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr int WAVES = 16;
 
-// OP: 0 v_mad_i64_i32 (+ arming v_mov) on 4 accumulator pairs, 1 v_pk_fma_f32 on 4 pairs, 2 v_add_u32 on 8 registers
+// OP: 0 v_mad_i64_i32 (+ arming v_mov) on 4 accumulator pairs, 2 v_add_u32 on 8 registers
 template <int K, int M, int OP, int DEP>
 __global__ __launch_bounds__(WAVES * 64) void k(unsigned trips, unsigned *out)
 {
@@ -22,11 +22,9 @@ __global__ __launch_bounds__(WAVES * 64) void k(unsigned trips, unsigned *out)
 	const unsigned at = (unsigned)(uintptr_t)mine + lane * 8u;
 	i32x2 v[K > 0 ? K : 1];
 	long long acc[4] = {1, 2, 3, 4};
-	f32x2 facc[4] = {{1.f, 2.f}, {3.f, 4.f}, {5.f, 6.f}, {7.f, 8.f}};
 	unsigned iacc[8] = {1, 2, 3, 4, 5, 6, 7, 8};
 	int x = (int)(tid * 77u + 5u), wgt = (int)(tid * 13u + 3u);
-	f32x2 fx = {1.0f + tid, 2.0f}, fw = {0.5f, 0.25f};
-	asm volatile("" : "+v"(x), "+v"(wgt), "+v"(fx), "+v"(fw));
+	asm volatile("" : "+v"(x), "+v"(wgt));
 #pragma unroll
 	for (int r = 0; r < K; ++r)
 		asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(v[r]) : "v"(at), "n"(r * 512));
@@ -61,8 +59,6 @@ __global__ __launch_bounds__(WAVES * 64) void k(unsigned trips, unsigned *out)
 				asm volatile("v_mad_i64_i32 %0, vcc, %1, %2, %0" : "+v"(a) : "v"(x), "v"(wgt) : "vcc");
 				acc[m & 3] = a;
 			}
-			else if constexpr (OP == 1)
-				asm volatile("v_pk_fma_f32 %0, %1, %2, %0" : "+v"(facc[m & 3]) : "v"(fx), "v"(fw));
 			else
 				asm volatile("v_add_u32 %0, %0, %1" : "+v"(iacc[m & 7]) : "v"(x));
 		}
@@ -70,7 +66,7 @@ __global__ __launch_bounds__(WAVES * 64) void k(unsigned trips, unsigned *out)
 	if constexpr (K > 0)
 		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 	for (int q = 0; q < 4; ++q)
-		sink ^= (unsigned)acc[q] ^ (unsigned)(acc[q] >> 32) ^ (unsigned)facc[q].x ^ (unsigned)facc[q].y;
+		sink ^= (unsigned)acc[q] ^ (unsigned)(acc[q] >> 32);
 	for (int q = 0; q < 8; ++q)
 		sink ^= iacc[q];
 	if (sink == 0xDEADBEEFu)
@@ -112,8 +108,6 @@ int main()
 	triple<15, 15, 0>("mov+mad_i64", d_out);
 	triple<15, 60, 0>("mov+mad_i64", d_out);
 	triple<8, 30, 0>("mov+mad_i64", d_out);
-	triple<15, 30, 1>("pk_fma_f32", d_out);
-	triple<15, 60, 1>("pk_fma_f32", d_out);
 	triple<15, 60, 2>("v_add_u32", d_out);
 	triple<15, 120, 2>("v_add_u32", d_out);
 	return 0;
