@@ -1168,6 +1168,24 @@ __device__ __forceinline__ void one_frame(const crhip_poly_launch &a, const int 
 }
 
 // ---------------------------------------------------------------------------------------------------------
+// One LDS read at byte address `at`, as ITS OWN instruction and where it stands among the others: volatile, so hipcc neither pairs it with a
+// neighbour (ds_read2_b64 moves 128 B per clock where ds_read_b64 moves 256) nor moves it across another such read.  hipcc knows what
+// is in flight and waits - counted, LDS returns in order - at the value's first use.  (Not inline assembly with waits of its own: hipcc
+// takes an asm statement's output as written on the spot and may copy the register before the data has landed.)
+// ---------------------------------------------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ T lds_read(unsigned at)
+{
+	return *(const volatile __attribute__((address_space(3))) T *)(uintptr_t)at;
+}
+// the value is here from this point on, and what follows in the source stays behind it
+template <typename T>
+__device__ __forceinline__ void landed(T &value)
+{
+	asm volatile("" : "+v"(value));
+}
+
+// ---------------------------------------------------------------------------------------------------------
 // Tickets, once per WAVE, from wave-uniform control flow with every lane active.  draw_ticket_begin: lane 0 adds 1 to the counter and
 // the value before the addition travels into a VGPR of the caller's; draw_ticket_end: the wave has it, in a scalar.
 // The atomic is a returning VECTOR instruction: it counts in vmcnt, with the wave's loads, LDS-DMA and stores, in issue order.  hipcc knows

@@ -35,16 +35,6 @@ namespace
 // loads cannot be made safe: hipcc copies their destination registers before the data has landed.)
 //   WAVES  waves per workgroup     NVW  1 KiB DMA pieces per wave-tile     ITER  frames per lane per wave-tile
 // ---------------------------------------------------------------------------------------------------------
-// LDS reads a frame has in flight BEHIND those of plane q while `ahead` planes are requested in advance: the planes q + 1 ...
-// q + ahead - 1 (a plane = the row vector, for the first channel pair, + one read per slot and channel read)
-constexpr int wave2_reads_ahead(bool with_rows, int reads_per_slot, int tt, int q, int ahead, int planes)
-{
-	int later = 0;
-	for (int g = q + 1; g < planes && g < q + ahead; ++g)
-		later += (with_rows ? 1 : 0) + reads_per_slot * ((tt - 4 * g) < 4 ? (tt - 4 * g) : 4);
-	return later;
-}
-
 // DUAL = 1: DUAL MONO (see k_poly): a stereo instance run on a MONO stream - output frames j and j + H, whose fractions are equal,
 // as its two channels.
 // ABL: 0 in every shipped instance.  Timing-only forms (WRONG results; built with -DCRA_WITH_W2_FORMS, reached through
@@ -556,7 +546,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_wave2(const crhip_poly_launch a)
 				i32x4 wq;
 				int x[4][CH];
 				i32x2 xv[4][(CH + 1) / 2];
-				asm volatile("ds_read_b128 %0, %1" : "=v"(wq) : "v"(row_q));
+				wq = lds_read<i32x4>(row_q);
 #pragma unroll
 				for (int s = 0; s < 4; ++s)
 				{
@@ -564,21 +554,17 @@ __global__ __launch_bounds__(WAVES * 64) void k_wave2(const crhip_poly_launch a)
 					for (int c = 0; c < CH; c += (EVEN ? 2 : 1))
 					{
 						if constexpr (EVEN)
-							asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(xv[s][c / 2]) : "v"(win_q), "n"((s * CH + c) * 4));
+							xv[s][c / 2] = lds_read<i32x2>(win_q + (unsigned)((s * CH + c) * 4));
 						else
-							asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(x[s][c]) : "v"(win_q), "n"((s * CH + c) * 4));
+							x[s][c] = lds_read<int>(win_q + (unsigned)((s * CH + c) * 4));
 					}
 				}
-				// the taps of slot s start when ITS reads have landed (in order: a counted wait), the later slots' under them
-				constexpr int READS_PER_SLOT = EVEN ? CH / 2 : CH;
-				asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(3 * READS_PER_SLOT < 15 ? 3 * READS_PER_SLOT : 15) : "memory");
-				asm volatile("" : "+v"(wq));
+				// the taps of slot s start when ITS reads have landed, the later slots' under them
+				landed(wq);
 				const int wv[4] = {wq.x, wq.y, wq.z, wq.w};
 #pragma unroll
 				for (int s = 0; s < 4; ++s)
 				{
-					if (s > 0)
-						asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"((3 - s) * READS_PER_SLOT < 15 ? (3 - s) * READS_PER_SLOT : 15) : "memory");
 #pragma unroll
 					for (int c = 0; c < CH; ++c)
 					{
@@ -586,13 +572,13 @@ __global__ __launch_bounds__(WAVES * 64) void k_wave2(const crhip_poly_launch a)
 						{
 							if (c % 2 == 0)
 							{
-								asm volatile("" : "+v"(xv[s][c / 2]));
+								landed(xv[s][c / 2]);
 								x[s][c] = xv[s][c / 2].x;
 								x[s][c + 1] = xv[s][c / 2].y;
 							}
 						}
 						else
-							asm volatile("" : "+v"(x[s][c]));
+							landed(x[s][c]);
 					}
 #pragma unroll
 					for (int c = 0; c < CH; ++c)
@@ -615,8 +601,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_wave2(const crhip_poly_launch a)
 			}
 #undef CRHIP_W2_TAPC
 			// (row_q now points at this row's entry in the plane after the weights: the reciprocal)
-			int reciprocal;
-			asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(reciprocal) : "v"(row_q) : "memory");
+			const int reciprocal = lds_read<int>(row_q);
 #pragma unroll
 			for (int c = 0; c < CH; ++c)
 			{
@@ -632,19 +617,15 @@ __global__ __launch_bounds__(WAVES * 64) void k_wave2(const crhip_poly_launch a)
 		int w[RS];
 		i32x4 wv[NQ];   // (the row reads land here)
 
-		// channels two at a time (the last one alone when CH is odd).  Every LDS read of the frame is issued up front - row plane q,
-		// then the window samples of its four slots, plane by plane - and the taps of plane q start as soon as ITS reads have
-		// landed (LDS returns in order: a counted lgkmcnt), the rest of the reads completing underneath the arithmetic.  All of
-		// them are inline assembly so that the counts are ours: hipcc's own waits only know the reads it issued itself.  Nothing
-		// may touch a destination register between its read and the "+v" statement behind the wait that covers it.
+		// channels two at a time (the last one alone when CH is odd): the LDS reads of the frame go out plane by plane - row plane q,
+		// then the window samples of its four slots - and the taps of plane q start as soon as ITS reads have landed.
 		static_for<(CH + 1) / 2>([&](auto c_tag) {
 			constexpr int c0 = 2 * decltype(c_tag)::value;
 			constexpr bool EVEN = CH % 2 == 0;
 			constexpr bool pair = c0 + 1 < CH;
 			constexpr int reads_per_slot = (pair && !EVEN) ? 2 : 1;
-			// The window as separate reads: left to itself hipcc pairs them into ds_read2_b64, which moves 128 B per clock where
-			// ds_read_b64 moves 256 (MI355X_MICROARCH.md, LDS) - and this kernel is as much LDS- as VALU-bound.  8-byte reads need
-			// 8-byte alignment: even channel counts only.
+			// The window as separate reads (lds_read): this kernel is as much LDS- as VALU-bound.  8-byte reads need 8-byte alignment:
+			// even channel counts only.
 			constexpr int TTN = TT > 0 ? TT : 1;   // (this part is never reached by the run-time-slot form; it still has to compile)
 			int xa[TTN], xb[TTN];
 			i32x2 xv[TTN];   // (the 8-byte reads land here)
@@ -662,33 +643,24 @@ __global__ __launch_bounds__(WAVES * 64) void k_wave2(const crhip_poly_launch a)
 					{
 						// pure upsampling has ONE row image whatever the ratio (UP_PLANE_ROWS rows per plane, checked at launch): the
 						// further planes are immediate offsets
-						asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(wv[q]) : "v"(row_at), "n"(q * (int)UP_PLANE_ROWS * 16));
+						wv[q] = lds_read<i32x4>(row_at + (unsigned)(q * (int)UP_PLANE_ROWS * 16));
 					}
 					else
+						wv[q] = lds_read<i32x4>(row_at + (unsigned)q * plane_bytes);
+				}
+#pragma unroll
+				for (int s = 4 * q; s < 4 * q + 4 && s < TT; ++s)
+				{
+					const unsigned at = win_at + (unsigned)((s * CH + c0) * 4);
+					if constexpr (pair && EVEN)
+						xv[s] = lds_read<i32x2>(at);
+					else
 					{
-						const unsigned at = row_at + (unsigned)q * plane_bytes;
-						asm volatile("ds_read_b128 %0, %1" : "=v"(wv[q]) : "v"(at));
+						xa[s] = lds_read<int>(at);
+						if constexpr (pair)
+							xb[s] = lds_read<int>(at + 4u);
 					}
 				}
-				// (four slots, written out: asm operands inside a further nested generic lambda do not capture for clang)
-#define CRHIP_W2_READ_SLOT(K)                                                                                                      \
-	if constexpr (4 * q + K < TT)                                                                                                  \
-	{                                                                                                                              \
-		constexpr int s = 4 * q + K;                                                                                               \
-		if constexpr (pair && EVEN)                                                                                                \
-			asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(xv[s]) : "v"(win_at), "n"((s * CH + c0) * 4));                      \
-		else                                                                                                                       \
-		{                                                                                                                          \
-			asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(xa[s]) : "v"(win_at), "n"((s * CH + c0) * 4));                      \
-			if constexpr (pair)                                                                                                    \
-				asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(xb[s]) : "v"(win_at), "n"((s * CH + c0 + 1) * 4));              \
-		}                                                                                                                          \
-	}
-				CRHIP_W2_READ_SLOT(0)
-				CRHIP_W2_READ_SLOT(1)
-				CRHIP_W2_READ_SLOT(2)
-				CRHIP_W2_READ_SLOT(3)
-#undef CRHIP_W2_READ_SLOT
 			};
 			// planes in flight: as many as 15 outstanding reads allow (a plane is a row vector + up to 4 x reads_per_slot reads)
 			constexpr int plane_reads_max = (c0 == 0 ? 1 : 0) + 4 * reads_per_slot;
@@ -702,37 +674,40 @@ __global__ __launch_bounds__(WAVES * 64) void k_wave2(const crhip_poly_launch a)
 			int lo0, hi0 = 0, lo1, hi1 = 0, lo2, hi2 = 0, lo3, hi3 = 0;
 			static_for<NQ>([&](auto q_tag) {
 				constexpr int q = decltype(q_tag)::value;
-				// reads issued after the last one of plane q - the planes ahead of it - may stay in flight
-				constexpr int later = wave2_reads_ahead(c0 == 0, reads_per_slot, TT, q, AHEAD, NQ);
-				static_assert(later <= 15, "lgkmcnt counts to 15");
-				asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(later) : "memory");
-				// (the plane that keeps AHEAD of them in flight, before the taps: its round trip runs under them)
-				if constexpr (q + AHEAD < NQ)
-					issue_plane(std::integral_constant<int, q + AHEAD>());
+				// plane q has landed - asked from its last read backwards: ONE wait, the planes ahead of it stay in flight - ...
+				constexpr int s_end = 4 * q + 4 < TT ? 4 * q + 4 : TT;
+#pragma unroll
+				for (int s = s_end - 1; s >= 4 * q; --s)
+				{
+					if constexpr (pair && EVEN)
+					{
+						landed(xv[s]);
+						xa[s] = xv[s].x;
+						xb[s] = xv[s].y;
+					}
+					else
+					{
+						if constexpr (pair)
+							landed(xb[s]);
+						else
+							xb[s] = 0;
+						landed(xa[s]);
+					}
+				}
 				if (c0 == 0)
 				{
-					asm volatile("" : "+v"(wv[q]));
+					landed(wv[q]);
 					w[4 * q] = wv[q].x;
 					w[4 * q + 1] = wv[q].y;
 					w[4 * q + 2] = wv[q].z;
 					w[4 * q + 3] = wv[q].w;
 				}
+				// ... and the plane that keeps AHEAD of them in flight goes out before the taps: its round trip runs under them
+				if constexpr (q + AHEAD < NQ)
+					issue_plane(std::integral_constant<int, q + AHEAD>());
 #pragma unroll
-				for (int s = 4 * q; s < 4 * q + 4 && s < TT; ++s)
+				for (int s = 4 * q; s < s_end; ++s)
 				{
-					if (pair && EVEN)
-					{
-						asm volatile("" : "+v"(xv[s]));
-						xa[s] = xv[s].x;
-						xb[s] = xv[s].y;
-					}
-					else if (pair)
-						asm volatile("" : "+v"(xa[s]), "+v"(xb[s]));
-					else
-					{
-						asm volatile("" : "+v"(xa[s]));
-						xb[s] = 0;
-					}
 					slot_taps(s, pair, xa[s], xb[s], w[s], lo0, hi0, lo1, hi1, lo2, hi2, lo3, hi3);
 				}
 			});

@@ -199,42 +199,41 @@ __global__ __launch_bounds__(1024) void k_wave2s(const crhip_poly_launch a)
 			i32x4 wq;
 			i32x2 xv[4];
 			int xa[4], xb[4];
-			asm volatile("ds_read_b128 %0, %1" : "=v"(wq) : "v"(row_q));
+			wq = lds_read<i32x4>(row_q);
 			if constexpr (EVENCH)
 			{
-				asm volatile("ds_read_b64 %0, %1" : "=v"(xv[0]) : "v"(win0));
-				asm volatile("ds_read_b64 %0, %1" : "=v"(xv[1]) : "v"(win1));
-				asm volatile("ds_read_b64 %0, %1" : "=v"(xv[2]) : "v"(win2));
-				asm volatile("ds_read_b64 %0, %1" : "=v"(xv[3]) : "v"(win3));
+				xv[0] = lds_read<i32x2>(win0);
+				xv[1] = lds_read<i32x2>(win1);
+				xv[2] = lds_read<i32x2>(win2);
+				xv[3] = lds_read<i32x2>(win3);
 			}
 			else
 			{
-				asm volatile("ds_read_b32 %0, %1" : "=v"(xa[0]) : "v"(win0));
-				asm volatile("ds_read_b32 %0, %1 offset:4" : "=v"(xb[0]) : "v"(win0));
-				asm volatile("ds_read_b32 %0, %1" : "=v"(xa[1]) : "v"(win1));
-				asm volatile("ds_read_b32 %0, %1 offset:4" : "=v"(xb[1]) : "v"(win1));
-				asm volatile("ds_read_b32 %0, %1" : "=v"(xa[2]) : "v"(win2));
-				asm volatile("ds_read_b32 %0, %1 offset:4" : "=v"(xb[2]) : "v"(win2));
-				asm volatile("ds_read_b32 %0, %1" : "=v"(xa[3]) : "v"(win3));
-				asm volatile("ds_read_b32 %0, %1 offset:4" : "=v"(xb[3]) : "v"(win3));
+				xa[0] = lds_read<int>(win0);
+				xb[0] = lds_read<int>(win0 + 4u);
+				xa[1] = lds_read<int>(win1);
+				xb[1] = lds_read<int>(win1 + 4u);
+				xa[2] = lds_read<int>(win2);
+				xb[2] = lds_read<int>(win2 + 4u);
+				xa[3] = lds_read<int>(win3);
+				xb[3] = lds_read<int>(win3 + 4u);
 			}
-			constexpr int RPS = EVENCH ? 1 : 2;   // reads per slot
-			asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(3 * RPS) : "memory");
-			asm volatile("" : "+v"(wq));
+			landed(wq);
 			const int wv[4] = {wq.x, wq.y, wq.z, wq.w};
 #pragma unroll
 			for (int s = 0; s < 4; ++s)
 			{
-				if (s > 0)
-					asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"((3 - s) * RPS) : "memory");
 				if constexpr (EVENCH)
 				{
-					asm volatile("" : "+v"(xv[s]));
+					landed(xv[s]);
 					xa[s] = xv[s].x;
 					xb[s] = xv[s].y;
 				}
 				else
-					asm volatile("" : "+v"(xa[s]), "+v"(xb[s]));
+				{
+					landed(xa[s]);
+					landed(xb[s]);
+				}
 				// (a padded slot has weight 0 and adds exactly 0 whatever its window read returns)
 				CRHIP_W2S_TAP(120, 121, lo0, hi0, xa[s], wv[s]);
 				CRHIP_W2S_TAP(122, 123, lo1, hi1, xb[s], wv[s]);
@@ -248,8 +247,7 @@ __global__ __launch_bounds__(1024) void k_wave2s(const crhip_poly_launch a)
 #undef CRHIP_W2S_TAP
 		(void)lo0;
 		(void)lo1;
-		int reciprocal;
-		asm volatile("ds_read_b32 %0, %1\n\ts_waitcnt lgkmcnt(0)" : "=v"(reciprocal) : "v"(row_q) : "memory");
+		const int reciprocal = lds_read<int>(row_q);
 		// (acc * reciprocal) / 32768 toward zero in 64 bits: right for either range class of the host's
 		const long long v0 = (long long)hi0 * (long long)reciprocal + (long long)((unsigned)(hi0 >> 31) >> 17);
 		const long long v1 = (long long)hi1 * (long long)reciprocal + (long long)((unsigned)(hi1 >> 31) >> 17);

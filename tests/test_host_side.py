@@ -530,6 +530,20 @@ def test_device_code_keeps_its_promises(tmp_path):
     assert draws >= 500 and counted >= 300, (draws, counted)   # every ticketed kernel; k_poly's tile loops
 
 
+def test_no_load_is_written_in_inline_assembly():
+    """hipcc takes an asm statement's output registers as written on the spot, and as free where nothing reads them: a load that is still in
+    flight behind its statement can land in a register that has been copied or given to something else.  The device code leaves
+    its loads to hipcc (lds_read, cr_device.hpp, where each has to stay an instruction of its own)."""
+    csrc = os.path.join(ROOT, "clownresampler_amd", "csrc")
+    found = []
+    for name in sorted(os.listdir(csrc)):
+        if name.endswith((".hip", ".hpp")):
+            for number, line in enumerate(open(os.path.join(csrc, name)), 1):
+                if re.search(r'"[^"]*\b(ds_read|ds_load|global_load|buffer_load|flat_load|scratch_load|s_load|s_buffer_load)', line.split("//")[0]):
+                    found.append("%s:%d" % (name, number))
+    assert not found, found
+
+
 REFERENCE = "/root/reference"
 
 

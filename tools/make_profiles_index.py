@@ -27,6 +27,7 @@ for doc in ("DESIGN.md", "README.md", "INTEGRATION.md"):
 cited.pop("INDEX.md", None)   # (this file)
 missing = [n for n in cited if not os.path.exists(os.path.join(P, n))]
 WHAT = [
+    (r"kwave2_lds_read_ab\.log", "`k_wave2` with its LDS reads as inline assembly and as volatile loads, same box"),
     (r"integer_chain_ratio_sweeps\.log", "`k_seg` and `k_up2` on integer chains against the other kernels by upsampling ratio; cfg 3 and its shorter forms (`bench.py`)"),
     (r"vector_tickets_all_workloads\.log", "every workload of bench.py once, tickets drawn by vector atomics"),
     (r"vector_tickets_ab\.log", "ticketed against round-robin tiles in `k_poly`, same box, three times each in turn"),
@@ -85,10 +86,10 @@ WHAT = [
     (r"r05_kwave2_lds_forms\.log", "timing-only forms of `k_wave2` (`hq44`, `dn8`, `hq48`): window / row reads without bank conflicts - the ceiling of the long-window shapes"),
     (r"r05_kwave2_frame_pipeline_ab\.log", "`k_wave2` with the frames of a wave-tile as one pipeline of LDS reads against frame by frame (bit-exact, ±1.5 %: not kept)"),
     (r"r05_kpoly_forms\.log", "timing-only forms of the headline `k_poly<2,5>`: compute floor, floor without bank conflicts, without stores; the int16 output by variant and tile size"),
-    (r"r05_ldswin\.log", "`tools/microbench/ldswin.hip`: LDS cycles per window slot by lane spacing for `ds_read_b64`, 8-byte-aligned and 16-byte-aligned `ds_read_b128`"),
+    (r"r05_ldswin\.log", "LDS cycles per window slot by lane spacing for `ds_read_b64`, 8-byte-aligned and 16-byte-aligned `ds_read_b128`"),
     (r"r05_mono_env_sweep\.log", "the host's rules against their environment overrides on the mono and mild-downsampling shapes (rotation, tile size, tickets, dual mono, lane order): no override beats the rule"),
     (r"r05_gpu_tests_last\.log", "`pytest -m gpu` with the long-stream tests added after the evidence run (same library build)"),
-    (r"r05_ldsvalu\.log", "`tools/microbench/ldsvalu.hip`: LDS reads and VALU work of a wave add up rather than overlap"),
+    (r"r05_ldsvalu\.log", "LDS reads and VALU work of a wave add up rather than overlap"),
     (r"r04_bench_cfg2\.json", "the headline `bench.py` line (BASELINE configs[1], N = 1) of the final build, with `roofline`, `cpu_baseline`, `parity_full_stream`, `strong_curve_n1`, `end_to_end`"),
     (r"r04_bench_(cfg3|cfg4|cfg5|hq48|cfg2_s16)\.json", "`bench.py` lines of the other workloads, same box and build"),
     (r"r04_bench_n\d_sharedgpu_gloo\.json", "`bench.py --gpus N` with the ranks SHARING one GPU over gloo (validation of the N > 1 path; not a scaling measurement)"),
