@@ -286,7 +286,7 @@ typedef struct cr_ring
 	int used;
 	unsigned next;
 	unsigned pending;            /* launches that have drawn a block of this ring and are not enqueued yet: hipStreamQuery
-	                                cannot see them, so a ring with any is never taken over (ADVICE r2) */
+	                                cannot see them, so a ring with any is never taken over */
 	unsigned long long last_use;
 } cr_ring;
 
@@ -483,7 +483,7 @@ int ClownResamplerAMD_DeviceCount(void)
 	return count;
 }
 
-/* Never reports through the error handler: this is the question a client asks BEFORE it commits to this library (VERDICT r4 item 9). */
+/* Never reports through the error handler: this is the question a client asks BEFORE it commits to this library. */
 int ClownResamplerAMD_IsUsable(void)
 {
 	crhip_device_info info;
@@ -538,7 +538,7 @@ static int host_free(void *pointer)
 /* Copies between the device and PAGEABLE host memory (the caller's buffers of the host-pointer entry points, the library's own malloc'ed
    images) go out in pieces of at most 1 MiB.  The runtime's answer to a larger one is to page-lock the host range IN PLACE (hsa_amd_memory_lock,
    device address == host address) and let the copy engine work on the caller's heap (profiles/r06_copy_path.txt: "HSA Copy Using Pinned
-   resource" above 1 MiB, "... Using Staging resource" up to it).  Every abort of a GPU test run that could be placed - three, rounds 5 and 6 -
+   resource" above 1 MiB, "... Using Staging resource" up to it).  Every abort of a GPU test run that could be placed - three -
    was a GPU page fault at an address inside the process's brk heap, reported while the main thread sat in such a copy (a 1.1-1.2 MB
    tensor.cpu() of the test), none of this library's launches having been given a host address (the flight recorder above).  What inside the
    runtime or the kernel driver goes wrong has not been established; what this library can do is keep ITS copies of a
@@ -978,7 +978,7 @@ int ClownResamplerAMD_ReserveCaptureLaunches(size_t launches)
 	return r != 0 ? -1 : 0;
 }
 
-/* The other end of the capture pool (ADVICE r2): a client that re-captures graphs over time says when the old ones are gone.
+/* The other end of the capture pool: a client that re-captures graphs over time says when the old ones are gone.
    Every block handed out to a captured launch on the current device becomes available again: the pool rewinds to its first
    chunk (zeroed again - a graph destroyed mid-flight could have left counters behind) and the later chunks are freed. */
 int ClownResamplerAMD_ReleaseCapturedLaunches(void)
@@ -1231,7 +1231,7 @@ static void fill_poly_launch(const ClownResamplerAMD_Plan *plan, crhip_poly_laun
 
 /* Variants from 1000 up are DIAGNOSTIC instances.  1006 ... 1008 compute what the kernel they stand for computes (they add clock stamps); the
    others are timing-only forms whose RESULTS ARE WRONG by design - those a shipped library never takes, whatever the environment says: only
-   a diagnostic build (make CRA_CFLAGS=-DCRA_WITH_W2_FORMS) accepts them (ADVICE r5). */
+   a diagnostic build (make CRA_CFLAGS=-DCRA_WITH_W2_FORMS) accepts them. */
 static int diagnostic_variant(int variant)
 {
 #ifdef CRA_WITH_W2_FORMS
@@ -1578,7 +1578,7 @@ static void plan_geometry(ClownResamplerAMD_Plan *plan)
 	if (tile >= 4u * frames_multiple)
 		tile = 4u * frames_multiple;
 	else if (tile >= 3u * frames_multiple && plan->channels <= 2u)
-		tile = 3u * frames_multiple;   /* (round 4: 48 -> 44.1 kHz fits three groups, not four: 2,048 -> 3,072-frame tiles; stereo + 4 %, and the
+		tile = 3u * frames_multiple;   /* (48 -> 44.1 kHz fits three groups, not four: 2,048 -> 3,072-frame tiles; stereo + 4 %, and the
 		                                  dual-mono launches on the stereo instance + 13 %; 4 and 8 channels measured 1-3 % SLOWER with three groups
 		                                  and keep two: profiles/r04_three_group_tiles_ab.log) */
 	else if (tile >= 2u * frames_multiple)
@@ -1915,7 +1915,7 @@ static int plan_seg_shape(const cr_device_ctx *ctx, ClownResamplerAMD_Plan *plan
 			image[r * 16u + 15u] = 2u * (uint32_t)row[plan->poly.slots];   /* the reciprocal, doubled: k_up2's normalisation (cr_kup.hpp) */
 		}
 		/* k_seg is an OPTIONAL fast path: whatever fails here leaves the plan without it (k_up2 / k_wave2 serve the configuration), and the
-		   store only ever holds an image that has arrived whole - a sibling plan must not find a pointer to rows nobody filled (ADVICE r5) */
+		   store only ever holds an image that has arrived whole - a sibling plan must not find a pointer to rows nobody filled */
 		void *rows = NULL;
 
 		failed = crhip_malloc(&rows, bytes) != 0;
@@ -2420,7 +2420,7 @@ int cr_plan_launch(const ClownResamplerAMD_Plan *plan, const void *d_in, uint64_
 		   the second half is the shorter one, its missing frames are computed on zeros / neighbours and not stored - less than one part
 		   in sixteen of the launch by the rule below, 0.1 % for ten minutes of audio. */
 		const ClownResamplerAMD_Plan *partner = plan->dual.partner;
-		/* (H a multiple of the period only: the last tile of the pairs may be a ragged one - round 4's first form rounded H to whole
+		/* (H a multiple of the period only: the last tile of the pairs may be a ragged one - the first form rounded H to whole
 		   tiles too, lcm(65536, 3072) = 196,608 frames for the 3-lobe instances, and took launches from 3.1 M output frames on) */
 		const uint64_t unit = plan->dual.period;
 		const uint64_t half = ((n_out + 1u) / 2u + unit - 1u) / unit * unit;
@@ -3087,7 +3087,7 @@ int ClownResamplerAMD_DebugHostIsDeviceVisible(const void *host, size_t bytes)
 
 /* The library at REST (no call in progress on any thread): what its process-wide state must look like then.  Waits for the devices it has
    touched, so every launch it ever enqueued has finished.  0 and an empty message when everything holds; otherwise the number of
-   findings, the first few in `message`.  (the reference has no globals; this library has - plan cache, ticket rings,
+   findings, the first few in `message`.  (The reference has no globals; this library has - plan cache, ticket rings,
    capture pool, staging sets, test hooks - and the GPU tests check after every test that they have returned to rest.) */
 int ClownResamplerAMD_DebugSelfCheck(char *message, size_t capacity)
 {

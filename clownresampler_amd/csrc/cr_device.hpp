@@ -554,7 +554,7 @@ __device__ __forceinline__ void store_shorts(short *dst, const int *v)
 // The FEWEST store instructions a lane's `bytes` contiguous output bytes can leave as: 16 per instruction.  This, not the number
 // of store statements in the source, is what a counted s_waitcnt vmcnt(N) behind a tile's stores may assume: hipcc merges
 // neighbouring stores (the 8 + 4 bytes of a 3-channel frame leave as ONE global_store_dwordx3), and a count larger than the
-// stores really outstanding no longer covers the LDS-DMA issued before them.  (Round 1 counted statements: with 3, 6 and 7
+// stores really outstanding no longer covers the LDS-DMA issued before them.  (Counting statements instead: with 3, 6 and 7
 // channels the wait was too weak - never seen with k_poly's long tiles, caught by k_wave2's short ones.)  A count that is too
 // small only waits for some of the tile's own stores as well.
 constexpr int min_stores_of_bytes(int bytes)
@@ -1219,7 +1219,7 @@ __device__ __forceinline__ unsigned draw_ticket_end(unsigned got)
 
 // ---------------------------------------------------------------------------------------------------------
 // SGPR budget.  Two 1024-thread workgroups per CU are 8 waves per SIMD, and on gfx950 a SIMD admits
-// min(8, 800 / (ceil(sgpr_count / 16) * 16 + 16)) waves (MI355X_MICROARCH.md, "Residency"): 8 only up to .sgpr_count 80,
+// min(8, 800 / (ceil(sgpr_count / 16) * 16 + 16)) waves: 8 only up to .sgpr_count 80,
 // 7 up to 96 - while the compiler's "Occupancy: 8" and hipOccupancyMaxActiveBlocksPerMultiprocessor still say 8 / two
 // workgroups.  Left alone hipcc gave most instances 82-106 SGPRs (wave-uniform 64-bit addresses, tile bookkeeping), so the
 // second workgroup of a CU only started when the first had finished - seen in the start ticks of the stamped diagnostic
@@ -1232,8 +1232,8 @@ __device__ __forceinline__ unsigned draw_ticket_end(unsigned got)
 // One architecture.  Several kernels drop stores that would land behind the caller's buffer by the RANGE CHECK of a raw buffer descriptor
 // with the per-store offset in the instruction's SCALAR offset operand (k_poly's and k_wave2's dual-mono stores, k_up2's copy-out,
 // k_seg's segments): on gfx9 / gfx950 the check is "offset >= num_records - soffset", the scalar offset included.  Other targets
-// leave it out of the check (LLVM's AMDGPU usage notes) and would write out of bounds - so this code is refused anywhere else
-// (ADVICE r4), and the guard-region tests (tests/test_gpu_parity.py: dual mono, test_segment_kernel_bit_exact) stay a mandatory gate.
+// leave it out of the check (LLVM's AMDGPU usage notes) and would write out of bounds - so this code is refused anywhere else,
+// and the guard-region tests (tests/test_gpu_parity.py: dual mono, test_segment_kernel_bit_exact) stay a mandatory gate.
 // ---------------------------------------------------------------------------------------------------------
 #if defined(__HIP_DEVICE_COMPILE__) && !defined(__gfx950__)
 #error "libclownresampler_amd's kernels are written for gfx950 (MI355X) only: see the note on buffer range checks above"

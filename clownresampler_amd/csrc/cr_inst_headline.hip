@@ -1,4 +1,4 @@
-// cr_inst_headline.hip - instance unit: mono / stereo with 3 lobes at 44.1 <-> 48 kHz ([4]) and the timing-only ablations of the headline instance  (see cr_instances.hpp)
+// cr_inst_headline.hip - instance unit: mono / stereo with 3 lobes at 44.1 <-> 48 kHz (the 10-minute and one-hour streams) and the timing-only ablations of the headline instance  (see cr_instances.hpp)
 #include "cr_instances.hpp"
 
 namespace crk

@@ -1,4 +1,4 @@
-// cr_inst_long.hip - instance unit: the 8-lobe build: 15- and 17-slot windows (stereo 8 -> 96 kHz through k_up)  (see cr_instances.hpp)
+// cr_inst_long.hip - instance unit: the 8-lobe build: 15- and 17-slot windows (stereo 8 -> 96 kHz through k_up2)  (see cr_instances.hpp)
 #include "cr_instances.hpp"
 
 namespace crk

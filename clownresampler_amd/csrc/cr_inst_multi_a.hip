@@ -1,4 +1,4 @@
-// cr_inst_multi_a.hip - instance unit: 8 channels 48 -> 44.1 kHz with every tuning variant (BASELINE configs[3])  (see cr_instances.hpp)
+// cr_inst_multi_a.hip - instance unit: 8 channels 48 -> 44.1 kHz with every tuning variant  (see cr_instances.hpp)
 #include "cr_instances.hpp"
 
 namespace crk

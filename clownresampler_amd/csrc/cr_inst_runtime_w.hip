@@ -3,7 +3,7 @@
 // to pay and fit a wave's slice of the LDS (cr_context.c plan_geometry)  (see cr_instances.hpp)
 #include "cr_instances.hpp"
 // k_wave2s (a lane per channel PAIR: cr_kwave2s.hpp) never became a default - it measured slower than the run-time-slot k_poly for the wide
-// frames it was written for (profiles/r03_wave2s.log) - so it is NOT in the default build any more (VERDICT r4 weak 10: a kernel nothing selects,
+// frames it was written for (profiles/r03_wave2s.log) - so it is NOT in the default build any more (a kernel nothing selects,
 // compiled into both libraries): `make CRA_CFLAGS=-DCRA_WITH_WAVE2S` brings it back behind variant 32 for comparison
 // (tests/test_gpu_parity.py::test_channel_pair_per_lane_kernel then runs instead of skipping).
 #ifdef CRA_WITH_WAVE2S

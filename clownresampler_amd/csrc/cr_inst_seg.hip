@@ -1,4 +1,4 @@
-// cr_inst_seg.hip - instance unit: k_seg (cr_kseg.hpp), the segment-per-lane kernel of long stereo 8-lobe upsampling launches (BASELINE configs[2])
+// cr_inst_seg.hip - instance unit: k_seg (cr_kseg.hpp), the segment-per-lane kernel of long stereo 8-lobe upsampling launches
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -20,7 +20,7 @@ struct seg_shape
 	unsigned chunk, groups, lds;
 };
 // (the timing-only forms exist in a diagnostic build only - make CRA_CFLAGS=-DCRA_WITH_W2_FORMS - so that nothing in the environment can make
-// a shipped library compute wrong samples, ADVICE r5; the stamped form computes what the kernel computes)
+// a shipped library compute wrong samples; the stamped form computes what the kernel computes)
 #ifdef CRA_WITH_W2_FORMS
 #define CR_SEG_FORM(abl) k_seg<15, 0x2A55u, SEG_WAVES, 1, 16u, 4u, abl>
 #else

@@ -29,7 +29,7 @@ namespace
 //           frames as two lanes of 4: every store instruction of a wave is one contiguous 1 KiB)
 // PH        1 = the frame has CH * SPLIT - 1 channels (odd totals above 8, SPLIT == 2): the second lane's last channel is a
 //           PHANTOM - it multiplies whatever follows the frame in the window and its result is never stored
-// DUAL      1 = DUAL MONO (round 4): a stereo instance run on a MONO stream.  Output frames j and j + H of one stream have the same
+// DUAL      1 = DUAL MONO: a stereo instance run on a MONO stream.  Output frames j and j + H of one stream have the same
 //           fractional position whenever H * increment is a multiple of 65536 - hence the same row - so they can be the two
 //           "channels" of one lane: one row index, one row read, one reciprocal for two frames, and the frame body is the stereo
 //           instance's, unchanged.  Per tile the two mono input windows (H * increment / 65536 input frames apart) are fetched by
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 	unsigned stamp_cycles = 0;
 	if constexpr (ABL == 6)
 	{
-		// diagnostic build only: in-kernel clock = cycles / (ticks / 100 MHz)  (MI355X_MICROARCH.md, DVFS give-back item 6).
+		// diagnostic build only: in-kernel clock = cycles / (ticks / 100 MHz).
 		// 32 bits of the cycle counter, and the start tick goes out at once: the instance has to stay at or below 96 SGPRs
 		// to be the same kernel as the one it stands for (see the note at `phase` below).
 		stamp_cycles = (unsigned)__builtin_amdgcn_s_memtime();
@@ -183,7 +183,7 @@ __global__ __launch_bounds__(NTHREADS) __attribute__((amdgpu_num_sgpr(CRHIP_SGPR
 	constexpr int STORES_PER_GROUP = PH ? U : (DUAL ? 2 * U : U * min_stores_of_bytes(CH * (OUT16 ? 2 : 4)));
 
 	// Tickets.  One global counter would serialise: a single word sustains ~88 atomic draws per microsecond on this
-	// chip (MI355X_MICROARCH.md, "dequeue") and a 10-minute stereo launch draws 7,000 of them - measured 92 us instead
+	// chip and a 10-minute stereo launch draws 7,000 of them - measured 92 us instead
 	// of 64.  So there are LANES counters (each on its own 128-byte line); the tiles are dealt round-robin to LANES
 	// sequences, workgroup b belongs to sequence b % LANES (workgroups b and b + 8 are observed to share an XCD, so with
 	// 8 lanes a sequence is mostly one XCD's - a speed matter only), starts with the tile of its own number and then

@@ -8,12 +8,12 @@ namespace
 {
 
 // ---------------------------------------------------------------------------------------------------------
-// k_seg - long upsampling launches (cfg 3: stereo 8 -> 96 kHz, 8 lobes), round 5
+// k_seg - long upsampling launches (cfg 3: stereo 8 -> 96 kHz, 8 lobes)
 // ---------------------------------------------------------------------------------------------------------
 // Where k_up2's time goes (profiles/r05_kup2_lds_ablations.log, timing-only builds): the row a lane reads for every frame - four
 // ds_read_b128, 64 bytes, 16 of a wave-step's ~34 LDS cycles, three VALU of addressing - is 18 % of the launch, and 64 lanes read
 // only four or five DIFFERENT rows per step.  The reference's position is j * increment in 16.16 (clownresampler.h:1076-1078), so
-// output frames j and j + S have the SAME fraction whenever S * increment is a multiple of 65536 (dual mono's observation, round 4):
+// output frames j and j + S have the SAME fraction whenever S * increment is a multiple of 65536 (dual mono's observation):
 // the same row, windows exactly D = S * increment / 65536 input frames apart.  Here the 64 lanes of a wave take the frames
 // j, j + S, ..., j + 63 S - lane l walks segment l of a "super-block" of 64 S output frames - so at every step the whole wave needs
 // ONE row, and:

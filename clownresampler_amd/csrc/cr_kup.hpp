@@ -431,7 +431,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_up(const crhip_poly_launch a)
 //     zero and a `lo` in [0, 65536] never does: hi += trunc(sample * weight / 65536), C's division (clownresampler.h:1020 via :625).
 //     |weight| << 15 needs |weight| < 65536: the two slots around the kernel's centre (mad_safemask<TT>(), weights up to 65536, never
 //     negative) keep the plain weight and take S = sample << 16 with the sign-shift arm B = S >> 31 - two registers per sample for
-//     those two slots only (round 2's form had S and B for all fifteen: 60 VALU per window and 60 registers; now 38 and 34).
+//     those two slots only (S and B for all fifteen would be 60 VALU per window and 60 registers: 38 and 34).
 //   * A frame's FIRST tap adds to a pinned pair {X of slot 0, 0}: no zeroing of the accumulator, no arming move for that tap.
 //   * The final (acc * reciprocal) / 32768 (clownresampler.h:1033) is one more 64-bit multiply-add on a pinned pair {bias, 0}
 //     and a funnel shift.
@@ -741,7 +741,7 @@ __global__ __launch_bounds__(WAVES * 64) void k_up2(const crhip_poly_launch a)
 			// v[126:127].  How a statement is DECLARED matters as much as what is in it: hipcc treats every asm statement as a
 			// possible forwarding hazard and pads with an s_nop whenever a register one statement DEFINES is touched - read or
 			// written - by the next instruction with nothing but other asm statements in between (15 s_nop per frame beside 73 VALU
-			// in round 3's first form, profiles/r03_kup2_nops.log).  So (1) the two chains take their carry-out in different
+			// in the first form, profiles/r03_kup2_nops.log).  So (1) the two chains take their carry-out in different
 			// registers, vcc and s[94:95], and may sit back to back; (2) a tap declares its low dword as an INPUT and a CLOBBER-free
 			// one: the multiply-add leaves the product's fraction bits there, which nothing ever reads - the next tap's arming move
 			// (hipcc's own instruction, free to follow the statement directly) overwrites it, and the last tap's is dead.  What

@@ -40,7 +40,7 @@ namespace
 // ABL: 0 in every shipped instance.  Timing-only forms (WRONG results; built with -DCRA_WITH_W2_FORMS, reached through
 // CLOWNRESAMPLER_AMD_W2_FORM): 1 = every lane reads the window of the wave-tile's first frame (window reads without bank conflicts),
 // 2 = every lane reads row 0 (row reads without), 3 = both.
-// (Tried in round 5 and NOT kept: the frames of a full wave-tile as ONE pipeline of LDS reads - the first planes of frame i + 1 requested
+// (Tried and NOT kept: the frames of a full wave-tile as ONE pipeline of LDS reads - the first planes of frame i + 1 requested
 // while the last planes of frame i are multiplied, into the registers those planes were consumed from; bit-exact, no extra registers -
 // within +-1.5 % of frame by frame on every shape, profiles/r05_kwave2_frame_pipeline_ab.log: the waves of a SIMD already cover each
 // other's round trips; what binds is the SUM of LDS and VALU cycles, profiles/r05_kwave2_lds_forms.log.)  The wave-tile's two mono windows are fetched into the two halves of the packed buffer by ONE descriptor

@@ -1,6 +1,6 @@
 /*
  * cr_multi.c - several GPUs behind the C ABI, one process: the output timeline of ONE stream split into contiguous blocks
- * (ClownResamplerAMD_PlanShard; SURVEY.md 8(e)), each block an ordinary low-level call on its own device and stream, and the
+ * (ClownResamplerAMD_PlanShard), each block an ordinary low-level call on its own device and stream, and the
  * optional final concatenate onto one device: peer copies (hipMemcpyPeerAsync: each peer -> root transfer is a point-to-point
  * copy over its own xGMI link) or RCCL's ncclGather (librccl is loaded on first use, never linked).
  * Host C; HIP through crhip.h only.  The reference has no counterpart (it has no threads and no devices); what is kept is
@@ -236,7 +236,7 @@ size_t cr_resample_sharded(ClownResampler_LowLevel_State *resampler, uint64_t ta
 	else if (gather_mode == CLOWNRESAMPLER_AMD_GATHER_RCCL)
 	{
 		/* Grouped point-to-point transfers with every shard's EXACT byte count (ncclGather wants one count from all ranks, which
-		   made the last and the empty shards' buffers part of a padding contract the library could not check: ADVICE r2): shard q
+		   made the last and the empty shards' buffers part of a padding contract the library could not check): shard q
 		   sends its block to the root, the root receives it at the block's place in the stream; the root's own block is a copy on
 		   its device.  NOT YET RUN with more than one rank - the pool's boxes have one GPU (tests/test_gpu_ranks.py
 		   test_two_distinct_gpus_over_rccl waits for a node that has two). */

@@ -1,6 +1,6 @@
 """Output-timeline sharding across ranks (one process per GPU, torch.distributed; backend "nccl" is RCCL on ROCm).
 
-The path shards trivially (SURVEY.md 8(e)): output frame k depends only on k, the configuration, the table and the input
+The path shards trivially: output frame k depends only on k, the configuration, the table and the input
 frames within `integer_stretched_kernel_radius` of its position.  Rank r therefore runs an ordinary low-level call on its
 slice of the input whose "padding" is the real neighbouring frames (which the reference allows, clownresampler.h:725-733)
 from the closed-form state at its first output frame - ClownResamplerAMD_PlanShard gives all of that.  There is NO

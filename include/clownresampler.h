@@ -7,9 +7,10 @@
  * (reference clownresampler.h:986-1035 driven by :1058-1092) runs as hand-written
  * HIP kernels on an AMD Instinct MI355X (gfx950).  There is no CPU fallback: if no
  * usable GPU / HIP runtime is present the library reports through the error handler
- * of clownresampler_amd.h, whose default prints the reason and aborts.
+ * of clownresampler_amd.h, whose default records and prints the reason and hands the
+ * failure back as "the callback said stop".
  *
- * How a client of the reference switches over (INTEGRATION.md has the details):
+ * How a client of the reference switches over:
  *   - keep its source unchanged; CLOWNRESAMPLER_IMPLEMENTATION / CLOWNRESAMPLER_STATIC
  *     are accepted and ignored (the reference's tests and examples define both,
  *     tests/test-low-level.c:25-28);

@@ -68,7 +68,7 @@ int ClownResamplerAMD_DeviceCount(void);                /* 0 when there is none;
    selection - else 0.  Never calls the error handler, never aborts: the question to ask ONCE, at start-up, by a client that wants to fall
    back on the reference's own header (clownresampler.h with CLOWNRESAMPLER_IMPLEMENTATION: same API, same results, one core) where
    there is no such device, instead of finding out from a failed first ClownResampler_*_Resample call.  This
-   library itself has no CPU path by design (INTEGRATION.md section 3). */
+   library itself has no CPU path by design. */
 int ClownResamplerAMD_IsUsable(void);
 int ClownResamplerAMD_SetDevice(int ordinal);           /* process default: device used by calls of threads that have not chosen one; 0 on success */
 int ClownResamplerAMD_SetThreadDevice(int ordinal);     /* device used by subsequent calls of the CALLING THREAD (-1: follow the process default again) */
@@ -309,7 +309,7 @@ size_t ClownResamplerAMD_ResampleSegmentsDevice(ClownResampler_LowLevel_State *r
                                                 void *device_output, size_t output_capacity_frames, int output_is_s16, size_t *segment_output_frames, void *hip_stream);
 
 /* ---------------------------------------------------------------------------------------------
- * Several GPUs, one process, one call (SURVEY.md 8(e); the reference has no counterpart).
+ * Several GPUs, one process, one call (the reference has no counterpart).
  * The output timeline of ONE stream is split into shard_count contiguous blocks (ClownResamplerAMD_PlanShard) and block r
  * is computed on shards[r].device, on shards[r].hip_stream: an ordinary low-level call on that shard's slice of the
  * input whose padding is the real neighbouring frames (clownresampler.h:725-733).  There is no exchange between the
@@ -319,7 +319,7 @@ size_t ClownResamplerAMD_ResampleSegmentsDevice(ClownResampler_LowLevel_State *r
  *   CLOWNRESAMPLER_AMD_GATHER_RCCL       EXPERIMENTAL: grouped ncclSend / ncclRecv over a communicator set of the shards' devices, exact
  *                                        sizes like the copies (librccl.so is loaded on first use; every ordinal may appear only
  *                                        once - checked before anything is launched).  It has only ever run with ONE rank (the
- *                                        test pool has single-GPU boxes), where no NCCL operation is issued at all: treat it as
+ *                                        machines it has run on have one GPU), where no NCCL operation is issued at all: treat it as
  *                                        unvalidated between distinct GPUs and prefer PEER_COPY until
  *                                        tests/test_gpu_ranks.py::test_two_distinct_gpus_over_rccl has run on a multi-GPU node.
  *                                        With MORE THAN ONE shard the call is refused (error ARGUMENT, nothing launched) unless

@@ -8,8 +8,8 @@
  * whose BEHAVIOUR it restates.  The arithmetic is kept scalar, one output
  * frame at a time, one integer divide per frame and one indirect call per
  * frame, so that timing it is representative of the reference C path
- * It is written from the behavioural description in
- * SURVEY.md, with 64-bit integers spelled out where the reference relies on
+ * It is written from a behavioural description of
+ * the reference, with 64-bit integers spelled out where the reference relies on
  * LP64 `long`.
  */
 #include "cr_oracle.h"
@@ -356,7 +356,7 @@ uint8_t oracle_high_end(oracle_highlevel *st, const int64_t *table, size_t table
 uint64_t oracle_count_output_frames(const oracle_lowlevel *st, uint64_t frames)
 {
 	/* frames are emitted while pos_int < frames, i.e. while P0 + j*inc < frames*65536
-	   (SURVEY.md section 8(a) a-2, verified against the reference by tests/test_oracle_vs_ref.py) */
+	   (verified against the reference by tests/test_oracle_vs_ref.py) */
 	const unsigned __int128 start = (unsigned __int128)st->pos_int * ORACLE_FRAC_ONE + st->pos_frac;
 	const unsigned __int128 limit = (unsigned __int128)frames * ORACLE_FRAC_ONE;
 
@@ -517,7 +517,7 @@ static void *mt_worker(void *arg)
 size_t oracle_low_resample_i32_mt(const oracle_lowlevel *fresh, const int64_t *table, size_t table_len,
                                   const int16_t *padded_in, size_t frames, int32_t *out, unsigned threads)
 {
-	/* contiguous input-frame ranges [a,b); start state from the closed form of SURVEY.md 8(d):
+	/* contiguous input-frame ranges [a,b); start state from the closed form:
 	   k0 = ceil(a*65536/inc), P = k0*inc, pos_int = (P >> 16) - a, pos_frac = P & 0xFFFF,
 	   pointer advanced by a frames (legal per clownresampler.h:725-733: the halo is real neighbours) */
 	mt_job *jobs;

@@ -80,7 +80,7 @@ typedef uint8_t (*oracle_output_cb)(void *user, const int64_t *frame, uint32_t s
 /* Normalisation variants.  CURRENT is what the shipped header does
  * (clownresampler.h:1025-1033).  LEGACY_GAIN replaces only that last step by a
  * constant 16.16 gain ratio(lowpass, in): it is what generated the reference's
- * stale goldens tests/test3 / tests/test4 (finding 1) and
+ * stale goldens tests/test3 / tests/test4 and
  * exists so those files can pin everything before the normalisation. */
 enum { ORACLE_NORM_CURRENT = 0, ORACLE_NORM_LEGACY_GAIN = 1 };
 
@@ -122,13 +122,13 @@ size_t oracle_low_resample_i32(oracle_lowlevel *st, const int64_t *table, size_t
 size_t oracle_high_run_i32(oracle_highlevel *st, const int64_t *table, size_t table_len, const int16_t *pcm,
                            size_t pcm_frames, size_t pull_chunk, int32_t *out, size_t out_capacity_frames);
 
-/* Stream hash of SURVEY.md section 8(d): h = (h ^ (uint64)(uint32)sample) * 1099511628211. */
+/* Stream hash: h = (h ^ (uint64)(uint32)sample) * 1099511628211. */
 uint64_t oracle_stream_hash(const int32_t *samples, size_t count, uint64_t seed);
 
-/* Synthetic PCM of SURVEY.md section 8(d): xorshift64 white noise, sample = (int16)(x >> 48). */
+/* Synthetic PCM: xorshift64 white noise, sample = (int16)(x >> 48). */
 uint64_t oracle_fill_noise(int16_t *dst, size_t samples, uint64_t state);
 
-/* Multi-threaded CPU baseline (BASELINE.md section 4): splits the input-frame
+/* Multi-threaded CPU baseline: splits the input-frame
  * range over `threads` independent states (closed-form start state), each
  * running oracle_low_resample through a storing callback.  out must hold
  * oracle_count_output_frames() frames.  Returns frames written. */

@@ -3,7 +3,7 @@
  * in place from /root/reference (never copied into this repo).
  *
  * TEST INFRASTRUCTURE ONLY.  Built by oracle/Makefile into
- * oracle/_ref/libclownref_r<R>.so (git-ignored, travels to the GPU box as a
+ * oracle/_ref/libclownref_r<R>.so (git-ignored, travels with the tree as a
  * prebuilt binary).  It plays the part tests/test-low-level.c:25-28 plays in the
  * reference: one translation unit that defines CLOWNRESAMPLER_IMPLEMENTATION +
  * CLOWNRESAMPLER_STATIC and includes the header, here by the path given on the
