@@ -2029,3 +2029,45 @@ def test_soak_short():
     trials, failures = soak_gpu.soak(45.0, 20261003, big_budget=True, log=lines.append)
     assert failures == 0, "\n".join(lines)
     assert trials >= 20, lines
+
+
+@pytest.mark.parametrize("radius,rates,kernel", [(8, (8000, 64000, 8000), 3), (8, (8000, 96000, 8000), 3), (8, (44100, 48000, 44100), 4)])
+def test_every_tile_is_taken_at_the_borders_of_the_dealing(products, radius, rates, kernel):
+    """The wave-tiles of k_up2 and the chunks of k_wave2 are dealt round-robin for all but the last two rounds and drawn as tickets from
+    there on.  Launches of whole rounds, one frame and one tile more and less, and of halves of a round: every frame against the oracle,
+    the frames behind the launch untouched, the ticket counters zero again for the launch that follows (the same plan, the same stream)."""
+    import torch
+    p, o = products[radius], ck.oracle(radius)
+    api = p.api
+    ch = 2
+    dev = torch.device("cuda", 0)
+    ok, ost = o.low_init(ch, *rates)
+    ok, st0 = p.low_init(ch, *rates)
+    plan = api.PlanCreate(st0.raw, p.pre)
+    info = api.PlanGetInfo(plan)
+    assert info.kernel == kernel
+    tile = info.tile_frames // 4
+    round_frames = info.max_blocks * (info.threads // 64) * tile
+    lengths = [max(k * round_frames // 2 + d, 1) for k in (7, 8, 9, 10) for d in (-tile, -1, 0, 1, tile)]
+    frames = (max(lengths) * rates[0]) // rates[1] + 64
+    R = int(ost.cfg.radius_frames)
+    padded = ck.pad_frames(ck.noise_pcm(frames * ch, 2024), ch, R)
+    want, _, _ = o.low_resample_i32(ost, padded, frames)
+    assert want.size // ch >= max(lengths)
+    d_in, d_want = torch.from_numpy(padded).to(dev), torch.from_numpy(want).to(dev)
+    d_out = torch.empty((max(lengths) + tile) * ch, dtype=torch.int32, device=dev)
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    api.DebugSegKernel(2)
+    try:
+        for n in lengths:
+            ok, st = p.low_init(ch, *rates)
+            d_out.fill_(0x5A5A5A5A)
+            takes = info.brief_kernel if n < info.brief_below else kernel   # (a short launch of a k_up2 plan takes its other kernel)
+            before = api.LaunchCount(takes)
+            got, left, ran_out = api.ResampleDevice(plan, st.raw, d_in.data_ptr(), frames, d_out.data_ptr(), n, stream)
+            torch.cuda.synchronize()
+            assert got == n and api.LaunchCount(takes) == before + 1, (n, got, takes)
+            assert torch.equal(d_out[:n * ch], d_want[:n * ch]), (rates, n, round_frames, tile)
+            assert bool((d_out[n * ch:] == 0x5A5A5A5A).all()), (rates, n, "frames behind the last one were written")
+    finally:
+        api.DebugSegKernel(0)
