@@ -237,12 +237,12 @@ def cpu_baseline(radius, ch, rates, frames, max_seconds=30.0):
 
 
 def pmc_summary(workload, build_id):
-    """Per-dispatch PMC means committed under profiles/ for this workload, latest round first: (dict, file name, note).  A summary
+    """Per-dispatch PMC means committed under profiles/ for this workload: (dict, file name, note).  A summary
     is quoted only when it is STAMPED with the source id of the library that is loaded now (tools/pmc_passes.sh writes
     ClownResamplerAMD_BuildId() into it): counters of another build say nothing about this one's kernels."""
     import glob
     stale = None
-    for path in sorted(glob.glob(os.path.join(ROOT, "profiles", "r[0-9][0-9]_%s_pmc_summary.txt" % workload)), reverse=True):
+    for path in sorted(glob.glob(os.path.join(ROOT, "profiles", "*_%s_pmc_summary.txt" % workload))):
         if os.path.exists(path):
             vals, stamp = {}, None
             for ln in open(path):
@@ -585,7 +585,7 @@ def main():
     # the same barrier bracket): straight after a barrier the chip has idled, and a 1.2 ms window (the driver's --steps 20 on cfg 2) caught
     # it 2-3 % above the sustained figure (mean of the first window 60.7 us against 62.6 us sustained on the same box).
     # With the queue kept full across ev0 the timed K launches run at the sustained clocks; `value` is that, and the rocprofv3 average
-    # over the timed dispatches (tools/r05_final_profiles.sh) reproduces it.
+    # over the timed dispatches (tools/evidence.sh) reproduces it.
     lead_in_launches = [0]
 
     def run_steps():

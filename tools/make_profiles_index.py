@@ -27,6 +27,11 @@ for doc in ("DESIGN.md", "README.md", "INTEGRATION.md"):
 cited.pop("INDEX.md", None)   # (this file)
 missing = [n for n in cited if not os.path.exists(os.path.join(P, n))]
 WHAT = [
+    (r"evidence_bench_.*\.json", "`bench.py` lines of the current build (`tools/evidence.sh`)"),
+    (r"evidence_.*_pmc_summary\.txt", "counters of the current build, stamped with its source id"),
+    (r"evidence_kernel_(stats|trace_head)_.*\.csv", "rocprofv3 kernel stats / the head of the trace of the same commands"),
+    (r"evidence_trace_timed_means\.log", "mean over exactly the timed dispatches, from the traces"),
+    (r"evidence_host_paths\.log", "host-pointer entry points and the callback signature (`tools/host_path_rate.py`)"),
     (r"kwave2_lds_read_ab\.log", "`k_wave2` with its LDS reads as inline assembly and as volatile loads, same box"),
     (r"integer_chain_ratio_sweeps\.log", "`k_seg` and `k_up2` on integer chains against the other kernels by upsampling ratio; cfg 3 and its shorter forms (`bench.py`)"),
     (r"vector_tickets_all_workloads\.log", "every workload of bench.py once, tickets drawn by vector atomics"),
